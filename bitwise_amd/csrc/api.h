@@ -306,4 +306,23 @@ int bw_moe_experts(const void* x, int x_is_bf16, int ldx, int x_rows, const void
 int bw_moe_tile_rows(int slots);
 int bw_moe_combine(const float* y, int ldy, const int32_t* place, const float* wts, int top, float* out, int ldo,
                    int rows, int width, int accumulate, void* stream);
+
+// ------------------------------------------------------------------------------ 8-bit rows and matrices
+// Rows of e4m3 codes [rows, ldq >= K rounded up to 128], zeros behind K, their scales at scales[block * lds + row]; see rows_fp8.h.
+// Codes and their strides are multiples of 16 bytes.
+int bw_quantize_fp8(const void* x, int x_is_bf16, int ldx, void* codes, int ldq, float* scales, int lds, int rows, int width, void* stream);
+// stream_out[r] = x[r] + scale * (gate * norm(y[r]) ), out[r] = norm(stream_out[r]): the norms around a sublayer, its gate and its
+// residual scale.  y null: out = norm(x).  post_weight null: y as it is; gate: [rows, dim] (ldg > 0), [dim] (ldg 0) or null,
+// through a sigmoid if asked; scale_vec [dim], or null: the number.  out_kind: 0 float, 1 bfloat16, 2 codes with ``scales``.
+int bw_norm_add_norm(const float* x, int ldx, const void* y, int y_is_bf16, int ldy, const void* post_weight, int post_is_bf16, float post_eps,
+                     const void* gate, int gate_is_bf16, int ldg, int gate_sigmoid, const void* scale_vec, int scale_is_bf16, float scale,
+                     float* stream_out, int ldst, const void* weight, int weight_is_bf16, float eps, void* out, int out_kind, int ldo,
+                     float* scales, int lds, int rows, int dim, void* stream);
+// out = x w^T (+ residual) of codes: w [N, K], ws [N rounded up to 128 / 128, K / 128], K whole blocks of 128.
+int bw_gemm_fp8(const void* x, int ldx, const float* xs, int ldxs, const void* w, const float* ws, const float* residual, int ldr, void* out,
+                int ldo, int out_is_bf16, int rows, int N, int K, void* stream);
+// codes, scales = quantized silu(g) u with [g | u] = x w^T: w [2 inter, K] (gate rows, then up rows), each half with scale blocks of
+// its own.  Up to 64 rows: ``sums`` [rows, inter] holds silu(g) u between two launches; more rows do not touch it.
+int bw_gemm_fp8_swiglu(const void* x, int ldx, const float* xs, int ldxs, const void* w, const float* ws, float* sums, int ldsums, void* codes,
+                       int ldq, float* scales, int lds, int rows, int inter, int K, void* stream);
 }

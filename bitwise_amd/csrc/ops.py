@@ -163,6 +163,13 @@ _SIGS = {
     "bw_moe_combine": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
     "bw_shared_key_attention": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int,
                                 c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p],
+    "bw_quantize_fp8": [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_void_p],
+    "bw_norm_add_norm": [c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int, c_float, c_void_p, c_int, c_int, c_int, c_void_p, c_int,
+                         c_float, c_void_p, c_int, c_void_p, c_int, c_float, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_void_p],
+    "bw_gemm_fp8": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                    c_void_p],
+    "bw_gemm_fp8_swiglu": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int,
+                           c_int, c_int, c_void_p],
 }
 
 _fns = {}
@@ -2008,6 +2015,205 @@ def moe_combine(y: torch.Tensor, place: torch.Tensor, wts: torch.Tensor, top: in
         raise ValueError("moe_combine: buffers do not fit")
     _check(_fn("bw_moe_combine")(y.data_ptr(), y.stride(0), place.data_ptr(), wts.data_ptr(), top, out.data_ptr(), out.stride(0),
                                  rows, out.shape[1], int(accumulate), _stream()), "moe_combine")
+
+
+# ------------------------------------------------------------------------------ 8-bit rows and matrices
+
+FP8 = torch.float8_e4m3fn
+FP8_BLOCK = 128                # elements of a row (rows and elements of a matrix) that share a scale
+FP8_SUMS_ROWS = 64             # rows up to which ``gemm_fp8_swiglu`` needs its buffer
+
+
+def fp8_width(width: int) -> int:
+    """The width of rows of codes: whole blocks."""
+    return -(-int(width) // FP8_BLOCK) * FP8_BLOCK
+
+
+def _need_rows(t: torch.Tensor, dtype, what: str) -> None:
+    """As ``_need_strided``, for matrices of one column too (whose column stride says nothing)."""
+    if not t.is_cuda:
+        raise ValueError(f"{what} must live on the GPU (there is no CPU path)")
+    if t.dtype != dtype:
+        raise ValueError(f"{what} must be {dtype}, got {t.dtype}")
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] != 1):
+        raise ValueError(f"{what} must be a matrix whose rows are contiguous")
+
+
+def _need_codes(codes: torch.Tensor, scales: torch.Tensor, rows: int, width: Optional[int], what: str) -> int:
+    """Rows of codes and their scales: [rows, whole blocks] e4m3 and [blocks, rows] float32, the rows of both contiguous;
+    returns the blocks."""
+    _need_rows(codes, FP8, f"{what}: codes")
+    _need_rows(scales, torch.float32, f"{what}: scales")
+    if width is not None and codes.shape[1] != fp8_width(width):
+        raise ValueError(f"{what}: codes of rows of {width} elements are {fp8_width(width)} wide, got {codes.shape[1]}")
+    if codes.shape[1] % FP8_BLOCK or codes.shape[1] == 0:
+        raise ValueError(f"{what}: rows of codes are whole blocks of {FP8_BLOCK}, got {codes.shape[1]}")
+    blocks = codes.shape[1] // FP8_BLOCK
+    if codes.shape[0] < rows or scales.shape[0] != blocks or scales.shape[1] < rows:
+        raise ValueError(f"{what}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} (blocks by rows) do not fit {rows} rows")
+    if codes.data_ptr() % 16 or (rows > 1 and codes.stride(0) % 16):
+        raise ValueError(f"{what}: rows of codes start at multiples of 16 bytes")
+    return blocks
+
+
+def _ld(t: Optional[torch.Tensor], rows: int) -> int:
+    """The stride of a matrix's rows (of a single row its width: the tensor's own says nothing)."""
+    return 0 if t is None else t.stride(0) if rows > 1 else t.shape[1]
+
+
+def _lb(scales: Optional[torch.Tensor]) -> int:
+    """The stride of rows' scales from block to block."""
+    return 0 if scales is None else _ld(scales, scales.shape[0])
+
+
+def _same_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1 or next(iter(devices)).index != torch.cuda.current_device():
+        raise ValueError(f"{what}: all tensors live on the current device")
+
+
+def quantize_fp8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, rows: int) -> None:
+    """x[:rows] (bfloat16 or float32, rows a stride apart) as e4m3 codes with a scale for each block of 128 elements of a row:
+
+        scales[b, r] = max(max |x[r, block b]|, 448 * 2^-126) / 448,  codes[r, k] = e4m3(x[r, k] * (1 / scales[b, r]))
+
+    all in 32 bits, the codes rounded to nearest even.  ``codes`` [>= rows, fp8_width(K)] gets zeros behind the rows' end;
+    ``scales`` [fp8_width(K) / 128, >= rows].  A block that holds an infinity or NaN stands for NaN throughout."""
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"quantize_fp8: x must be bfloat16 or float32, got {x.dtype}")
+    _need_rows(x, x.dtype, "quantize_fp8: x")
+    _need_codes(codes, scales, rows, x.shape[1], "quantize_fp8")
+    if x.shape[0] < rows:
+        raise ValueError("quantize_fp8: x is shorter than the rows")
+    _same_device("quantize_fp8", x, codes, scales)
+    _check(_fn("bw_quantize_fp8")(x.data_ptr(), _is_bf16(x, "x"), _ld(x, rows), codes.data_ptr(), _ld(codes, rows), scales.data_ptr(), _lb(scales),
+                                  rows, x.shape[1], _stream()), "quantize_fp8")
+
+
+def norm_add_norm(x: torch.Tensor, y: Optional[torch.Tensor], weight: torch.Tensor, out: torch.Tensor, rows: int, eps: float,
+                  post_weight: Optional[torch.Tensor] = None, post_eps: Optional[float] = None, gate: Optional[torch.Tensor] = None,
+                  gate_sigmoid: bool = False, scale=1.0, stream: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None) -> None:
+    """The norms around a sublayer, its gate and its residual scale in one launch, all 32-bit:
+
+        z = norm(y) * post_weight (without ``post_weight``: y),  z *= gate, or its sigmoid
+        stream = x + scale * z,  out = norm(stream) * weight
+
+    with norm(v) = v / sqrt(mean(v^2) + eps) (``post_eps`` for the first one, ``eps`` if not given).  x [rows, dim] float32; y
+    bfloat16 or float32; ``gate`` [rows, dim] or [dim], ``scale`` a number or a vector [dim], the weights [dim]: bfloat16 or
+    float32 each.  ``stream`` (float32) may be x and is x if not given.  ``out`` is float32, bfloat16 (one rounding) or e4m3
+    codes [rows, fp8_width(dim)] with ``scales`` as ``quantize_fp8`` of the 32-bit rows gives them.  y None: out = norm(x) *
+    weight, and nothing else is given."""
+    _need_rows(x, torch.float32, "norm_add_norm: x")
+    dim = x.shape[1]
+
+    def vector(t, what):
+        if t is None:
+            return None, 0
+        if t.dim() != 1 or t.shape[0] != dim or not t.is_cuda or not t.is_contiguous():
+            raise ValueError(f"norm_add_norm: {what} must be a contiguous vector of {dim} on the GPU")
+        return t.data_ptr(), _is_bf16(t, what)
+
+    def matrix(t, what):
+        _need_rows(t, t.dtype, f"norm_add_norm: {what}")
+        if t.shape[0] < rows or t.shape[1] != dim:
+            raise ValueError(f"norm_add_norm: {what} {tuple(t.shape)} does not fit {rows} rows of {dim}")
+        return t.data_ptr(), _is_bf16(t, what), _ld(t, rows)
+
+    if x.shape[0] < rows:
+        raise ValueError("norm_add_norm: x is shorter than the rows")
+    scale_vec = scale if isinstance(scale, torch.Tensor) else None
+    if y is None and not (post_weight is None and gate is None and stream is None and scale_vec is None and scale == 1.0):
+        raise ValueError("norm_add_norm: without a sublayer's output there is nothing to norm, gate, scale or add")
+    if stream is None and y is not None:
+        stream = x
+    if stream is not None:
+        _need_rows(stream, torch.float32, "norm_add_norm: stream")
+        if stream.shape[0] < rows or stream.shape[1] != dim:
+            raise ValueError(f"norm_add_norm: stream {tuple(stream.shape)} does not fit {rows} rows of {dim}")
+    if (scales is not None) != (out.dtype == FP8):
+        raise ValueError("norm_add_norm: codes come with scales, other rows without")
+    if out.dtype == FP8:
+        _need_codes(out, scales, rows, dim, "norm_add_norm")
+        kind, ldo = 2, _ld(out, rows)
+    else:
+        _, kind, ldo = matrix(out, "out")
+    yp, yb, ldy = (None, 0, 0) if y is None else matrix(y, "y")
+    if gate is None:
+        gp, gb, ldg = None, 0, 0
+    elif gate.dim() == 2:
+        gp, gb, ldg = matrix(gate, "gate")
+        if ldg == 0:
+            raise ValueError("norm_add_norm: a gate for all rows is a vector")
+    else:
+        gp, gb = vector(gate, "gate")
+        ldg = 0
+    pp, pb = vector(post_weight, "post_weight")
+    sp, sb = vector(scale_vec, "scale")
+    wp, wb = vector(weight, "weight")
+    _same_device("norm_add_norm", x, y, weight, out, post_weight, gate, scale_vec, stream, scales)
+    _check(_fn("bw_norm_add_norm")(x.data_ptr(), _ld(x, rows), yp, yb, ldy, pp, pb, float(eps if post_eps is None else post_eps), gp, gb, ldg,
+                                   int(bool(gate_sigmoid)), sp, sb, 0.0 if scale_vec is not None else float(scale),
+                                   None if stream is None else stream.data_ptr(), _ld(stream, rows), wp, wb, float(eps),
+                                   out.data_ptr(), kind, ldo, None if scales is None else scales.data_ptr(), _lb(scales),
+                                   rows, dim, _stream()), "norm_add_norm")
+
+
+def _need_fp8_matrix(w: torch.Tensor, w_scales: torch.Tensor, halves: int, blocks: int, what: str) -> int:
+    """A matrix [halves * N, K] of codes with its scales; returns N."""
+    _need(w, FP8, f"{what}: weight")
+    _need(w_scales, torch.float32, f"{what}: weight scales")
+    if w.dim() != 2 or w.shape[0] % halves or w.shape[0] == 0:
+        raise ValueError(f"{what}: weight must be a matrix" + (" of gate rows, then as many up rows" if halves == 2 else ""))
+    n = w.shape[0] // halves
+    if w.shape[1] != blocks * FP8_BLOCK or tuple(w_scales.shape) != (halves * (-(-n // FP8_BLOCK)), blocks):
+        raise ValueError(f"{what}: weight {tuple(w.shape)} with scales {tuple(w_scales.shape)} does not fit rows of {blocks} blocks of {FP8_BLOCK}")
+    return n
+
+
+def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, rows: int,
+             residual: Optional[torch.Tensor] = None) -> None:
+    """out[:rows] = x[:rows] @ w.T (+ residual) for rows and a matrix of e4m3 codes: ``x``, ``x_scales`` as ``quantize_fp8`` leaves them,
+    ``w`` [N, fp8_width(K)] with zeros behind K and ``w_scales`` [ceil(N / 128), fp8_width(K) / 128], a scale for each 128 x 128
+    block.  Each block's products are summed in 32 bits, the blocks' sums times their two scales are added up in 32 bits, k
+    ascending: a row's bits do not depend on the rows beside it.  ``out`` is float32 or bfloat16 (one rounding), its rows a stride
+    apart; ``residual`` (float32, with a float32 ``out``, which it may be) is added last."""
+    blocks = _need_codes(x, x_scales, rows, None, "gemm_fp8")
+    n = _need_fp8_matrix(w, w_scales, 1, blocks, "gemm_fp8")
+    bf16 = _is_bf16(out, "out")
+    _need_rows(out, out.dtype, "gemm_fp8: out")
+    if out.shape[0] < rows or out.shape[1] != n:
+        raise ValueError(f"gemm_fp8: out {tuple(out.shape)} does not fit {rows} rows of {n}")
+    if residual is not None:
+        _need_rows(residual, torch.float32, "gemm_fp8: residual")
+        if bf16 or residual.shape[0] < rows or residual.shape[1] != n:
+            raise ValueError("gemm_fp8: a residual has out's width, and out is 32-bit then")
+    _same_device("gemm_fp8", x, x_scales, w, w_scales, out, residual)
+    _check(_fn("bw_gemm_fp8")(x.data_ptr(), _ld(x, rows), x_scales.data_ptr(), _lb(x_scales), w.data_ptr(), w_scales.data_ptr(),
+                              None if residual is None else residual.data_ptr(), _ld(residual, rows),
+                              out.data_ptr(), _ld(out, rows), bf16, rows, n, x.shape[1], _stream()), "gemm_fp8")
+
+
+def gemm_fp8_swiglu(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, codes: torch.Tensor,
+                    scales: torch.Tensor, rows: int, sums: Optional[torch.Tensor] = None) -> None:
+    """codes, scales [:rows] = ``quantize_fp8`` of silu(g) * u with [g | u] = x @ w.T as ``gemm_fp8`` computes it: a feed-forward's first half,
+    ready for the product with its down projection.  ``w`` [2N, K] holds the gate rows, then the up rows, each half with scale
+    blocks of its own: ``w_scales`` [2 ceil(N / 128), K / 128].  More than 64 rows: one launch, whose epilogue does it all; up to 64
+    rows need ``sums`` (float32 [>= rows, N]), where silu(g) * u lies between two launches.  The bits are the same either way."""
+    blocks = _need_codes(x, x_scales, rows, None, "gemm_fp8_swiglu")
+    n = _need_fp8_matrix(w, w_scales, 2, blocks, "gemm_fp8_swiglu")
+    _need_codes(codes, scales, rows, n, "gemm_fp8_swiglu")
+    if rows <= FP8_SUMS_ROWS:
+        if sums is None:
+            raise ValueError(f"gemm_fp8_swiglu: up to {FP8_SUMS_ROWS} rows need a buffer for their sums")
+        _need_rows(sums, torch.float32, "gemm_fp8_swiglu: sums")
+        if sums.shape[0] < rows or sums.shape[1] != n:
+            raise ValueError(f"gemm_fp8_swiglu: sums {tuple(sums.shape)} do not fit {rows} rows of {n}")
+    else:
+        sums = None
+    _same_device("gemm_fp8_swiglu", x, x_scales, w, w_scales, codes, scales, sums)
+    _check(_fn("bw_gemm_fp8_swiglu")(x.data_ptr(), _ld(x, rows), x_scales.data_ptr(), _lb(x_scales), w.data_ptr(), w_scales.data_ptr(),
+                                     None if sums is None else sums.data_ptr(), _ld(sums, rows), codes.data_ptr(),
+                                     _ld(codes, rows), scales.data_ptr(), _lb(scales), rows, n, x.shape[1], _stream()), "gemm_fp8_swiglu")
 
 
 # ------------------------------------------------------------------------------ sampling

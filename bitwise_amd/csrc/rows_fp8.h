@@ -1,0 +1,109 @@
+// Rows as e4m3 codes with a 32-bit scale for each block of 128 elements: what the kernels that leave such rows share
+// (quantize_fp8.hip, gemm_fp8.hip).  A row of K elements has whole blocks of codes, zeros behind its end; the scale of block b
+// of row r lies at scales[b * ld + r], block by block, so that a product's 16 rows find a block's scales side by side.
+//
+//   scale = max(max |x|, 448 * 2^-126) / 448,  code = e4m3(x * (1 / scale)), rounded to nearest even
+//
+// with the division and the reciprocal correctly rounded: a block of zeros has the scale 2^-126, no quotient overflows (the
+// largest magnitude gives 448 within two units in the last place, and 448 is what all up to 464 round to), and every
+// route to a row gives the same bits.  A block with an infinity or NaN has an infinite or NaN scale: everything in it stands for NaN.
+#pragma once
+
+#include "common.h"
+
+#define BW_FP8_BLOCK 128
+
+// The largest of non-negative floats by their bits, which puts NaN above infinity (a float maximum would drop it).
+__device__ __forceinline__ uint32_t max_bits(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+// over the 16 lanes of a row of lanes
+__device__ __forceinline__ uint32_t row16_max_bits(uint32_t v) {
+  v = max_bits(v, __float_as_uint(lane_xor<8>(__uint_as_float(v))));
+  v = max_bits(v, __float_as_uint(lane_xor<4>(__uint_as_float(v))));
+  v = max_bits(v, __float_as_uint(lane_xor<2>(__uint_as_float(v))));
+  return max_bits(v, __float_as_uint(lane_xor<1>(__uint_as_float(v))));
+}
+
+__device__ __forceinline__ float fp8_scale_of(uint32_t amax_bits) {
+  return __uint_as_float(max_bits(amax_bits, __float_as_uint(448.0f * 0x1p-126f))) / 448.0f;
+}
+
+// Four codes of four values times the scale's reciprocal.
+__device__ __forceinline__ uint32_t fp8_codes4(float a, float b, float c, float d, float inv) {
+  int v = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, v, true);
+}
+
+// Eight consecutive elements as they come from memory: 16 bytes of bfloat16 or 32 of floats.  The load is a step of its own, so
+// that a caller can ask for everything before anything is waited for.
+struct Raw8 {
+  u32x4 a, b;
+};
+
+// Elements e .. e + 7 of ``p``, those from ``end`` on as zeros.  VEC: 16-byte loads (aligned, ``end`` a multiple of 8);
+// otherwise one element at a time, left as floats.
+template <bool VEC>
+__device__ __forceinline__ Raw8 load_raw8(const void* p, int is_bf16, size_t row_at, int e, int end) {
+  Raw8 r;
+  r.a = r.b = (u32x4){0u, 0u, 0u, 0u};
+  if constexpr (VEC) {
+    if (e < end) {
+      if (is_bf16) {
+        r.a = *reinterpret_cast<const u32x4*>((const bf16_t*)p + row_at + e);
+      } else {
+        r.a = *reinterpret_cast<const u32x4*>((const float*)p + row_at + e);
+        r.b = *reinterpret_cast<const u32x4*>((const float*)p + row_at + e + 4);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t v = 0u;
+      if (e + i < end) v = is_bf16 ? (uint32_t)((const bf16_t*)p)[row_at + e + i] << 16 : ((const uint32_t*)p)[row_at + e + i];
+      if (i < 4) r.a[i] = v;
+      else r.b[i - 4] = v;
+    }
+  }
+  return r;
+}
+
+template <bool VEC>
+__device__ __forceinline__ void raw8_floats(const Raw8& r, int is_bf16, float (&v)[8]) {
+  if (VEC && is_bf16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(r.a[i] << 16);
+      v[2 * i + 1] = __uint_as_float(r.a[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = __uint_as_float(r.a[i]);
+      v[4 + i] = __uint_as_float(r.b[i]);
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t largest8(const float (&v)[8]) {
+  uint32_t m = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max_bits(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  return m;
+}
+
+// 1 / (1 + exp(-g)) within two units in the last place: codes are rounded from it, and what is more off moves more of them to
+// a neighbour.  The exponential through the hardware exp2, its argument in two parts; the quotient through the hardware
+// reciprocal and one Newton step.  (Below -88 the argument stays there: the result is under 10^-38.)  NaN gives a number.
+__device__ __forceinline__ float sigmoid_of_number(float g) {
+  const float x = fminf(-g, 88.0f);
+  const float hi = x * 0x1.715476p+0f;
+  const float lo = fmaf(x, 0x1.715476p+0f, -hi) + x * 0x1.4ae0cp-26f;
+  const float d = fmaf(__builtin_amdgcn_exp2f(hi), fmaf(lo, 0x1.62e43p-1f, 1.0f), 1.0f);
+  const float r = __builtin_amdgcn_rcpf(d);
+  return fmaf(fmaf(-d, r, 1.0f), r, r);
+}
+
+__device__ __forceinline__ float sigmoid32(float g) { return g != g ? g : sigmoid_of_number(g); }
+
+// silu(g) u (a NaN goes through the first product)
+__device__ __forceinline__ float silu32_times(float g, float u) { return (g * sigmoid_of_number(g)) * u; }
