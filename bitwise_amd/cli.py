@@ -145,7 +145,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     r.add_argument("--config", required=True, help="a config.json")
     r.add_argument("--seed", type=int, default=0)
     r.add_argument("--sigma", type=float, default=0.02, help="standard deviation of linear and embedding weights")
-    r.add_argument("--weight-dtype", choices=["bfloat16", "float32", "float16"], default="bfloat16")
+    r.add_argument("--weight-dtype", choices=["bfloat16", "float32", "float16", "float8"], default="bfloat16")
     r.add_argument("--out", required=True)
 
     args = ap.parse_args(argv)

@@ -5,7 +5,8 @@ architecture name is ``architectures[0]``, ``num_key_value_heads`` defaults to t
 number of heads, ``head_dim`` to ``hidden_size // num_attention_heads``,
 ``rope_theta`` to 10000.0, ``rms_norm_eps`` to 1e-6, ``tie_word_embeddings`` to
 False, a list ``eos_token_id`` means its first element, and a truthy
-``rope_scaling`` is refused (tools/convert.py:59-60).  ``max_position_embeddings``
+``rope_scaling`` is refused (tools/convert.py:59-60), and so is a
+``quantization_config`` of another form than 8-bit codes with a scale for each block of 128 x 128.  ``max_position_embeddings``
 is not read by the reference; here it bounds the rotary table and request lengths.
 """
 
@@ -79,6 +80,11 @@ class LlamaConfig:
         for key in ("attention_bias", "mlp_bias"):
             if d.get(key):
                 raise ConfigError(f"{key}=true is not supported by the Llama parts of this engine")
+        quantized = d.get("quantization_config")
+        if quantized and (quantized.get("quant_method") != "fp8" or quantized.get("fmt", "e4m3") != "e4m3"
+                          or quantized.get("activation_scheme", "dynamic") != "dynamic" or list(quantized.get("weight_block_size") or []) != [128, 128]):
+            raise ConfigError("quantization_config: matrices in 8 bits are e4m3 codes with a scale for each block of 128 x 128 (quant_method "
+                              f"'fp8', weight_block_size [128, 128], inputs quantized as they come), got {dict(quantized)}")
         act = d.get("hidden_act", "silu")
         if act != "silu":
             raise ConfigError(f"hidden_act '{act}' is not supported; the feed-forward is SwiGLU with SiLU")

@@ -19,7 +19,7 @@ from . import registry
 from .models.assembled import AssembledModel
 from .parts.base import TensorSpec
 from .runtime import Runtime
-from .weights import loader
+from .weights import block_scaled, loader
 
 
 def model_spec(config: Mapping[str, Any]):
@@ -37,10 +37,11 @@ def write_random_model(folder: str | Path, config: Mapping[str, Any], seed: int,
                        dtype: str = "bfloat16") -> Path:
     """Random-weights mode: writes ``config.json`` and ``model.safetensors`` into ``folder``.
     Linear and embedding weights are N(0, sigma), norm weights 1 + N(0, 0.1), drawn in the
-    model's tensor order from one generator seeded with ``seed``."""
+    model's tensor order from one generator seeded with ``seed``.  dtype "float8": matrices of the parts that take them so are stored
+    in 8 bits with a scale for each block of 128 x 128, the rest in bfloat16."""
     arch = registry.architecture_of(config)
     typed = arch.config_from_dict(config)
-    torch_dtype = {"bfloat16": torch.bfloat16, "float32": torch.float32, "float16": torch.float16}[dtype]
+    torch_dtype = {"bfloat16": torch.bfloat16, "float32": torch.float32, "float16": torch.float16, "float8": block_scaled.DTYPE}[dtype]
     return loader.write_model_folder(folder, typed.to_dict(), describe(config), seed, sigma, torch_dtype)
 
 
@@ -82,14 +83,15 @@ class Model:
         assembled = AssembledModel(arch.spec_from_config(typed), rt)
         gen = torch.Generator(device=rt.device)
         gen.manual_seed(int(seed))
-        wd = {"bfloat16": torch.bfloat16, "float32": torch.float32}[weight_dtype]
+        wd = {"bfloat16": torch.bfloat16, "float32": torch.float32, "float8": block_scaled.DTYPE}[weight_dtype]
         tensors = {}
         for name, ts in assembled.tensor_specs().items():
             if ts.kind == "int":
                 tensors[name] = loader.random_table(ts, gen, rt.device)
                 continue
             z = torch.randn(ts.shape, generator=gen, dtype=torch.float32, device=rt.device)
-            tensors[name] = loader.shape_values(ts.kind, z, sigma).to(wd)
+            stored = [t for _, t in loader.stored_as(name, ts, loader.shape_values(ts.kind, z, sigma), wd)]
+            tensors[name] = stored[0] if len(stored) == 1 else block_scaled.BlockScaled([tuple(stored)], ts.shape[1])
         assembled.bind_tensors(tensors)
         return cls(typed, assembled)
 

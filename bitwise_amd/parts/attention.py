@@ -16,6 +16,7 @@ import numpy as np
 import torch
 
 from ..csrc import ops
+from ..weights.block_scaled import stacked
 from .base import CacheSpec, Mixer, TensorSpec, lookup, register_mixer, POSITION_ENCODINGS
 from .linear import Linear
 
@@ -211,10 +212,10 @@ class Attention(Mixer):
 
     def tensors(self) -> Dict[str, TensorSpec]:
         return {
-            "q_proj.weight": TensorSpec((self.q_dim, self.width)),
-            "k_proj.weight": TensorSpec((self.kv_dim, self.width)),
-            "v_proj.weight": TensorSpec((self.kv_dim, self.width)),
-            "o_proj.weight": TensorSpec((self.width, self.q_dim)),
+            "q_proj.weight": TensorSpec((self.q_dim, self.width), block_scaled=True),
+            "k_proj.weight": TensorSpec((self.kv_dim, self.width), block_scaled=True),
+            "v_proj.weight": TensorSpec((self.kv_dim, self.width), block_scaled=True),
+            "o_proj.weight": TensorSpec((self.width, self.q_dim), block_scaled=True),
         }
 
     def _tables(self):
@@ -238,7 +239,7 @@ class Attention(Mixer):
         q, k, v = tensors["q_proj.weight"], tensors["k_proj.weight"], tensors["v_proj.weight"]
         if not (q.dtype == k.dtype == v.dtype):
             raise ValueError("q, k and v projections must be stored in one dtype to be stacked")
-        self.qkv = Linear(torch.cat([q, k, v], dim=0), self.rt)
+        self.qkv = Linear(stacked([q, k, v]), self.rt)
         self.o = Linear(tensors["o_proj.weight"], self.rt)
 
     def weight_bytes(self) -> int:
@@ -255,6 +256,14 @@ class Attention(Mixer):
         """Decode steps of few rows: norm, q|k|v product, rotation and cache write are one kernel."""
         from .norm import RMSNorm
         rt, ws = self.rt, ctx.ws
+        if self.qkv.fp8 and type(norm) is RMSNorm:
+            # (any number of rows: the normed rows are in 8 bits at once, whatever step they are in)
+            codes, scales = self.qkv.codes(ws)
+            ops.norm_add_norm(x, None, norm.weight, codes, ctx.rows, norm.eps, scales=scales)
+            qkv = ws.buffer("qkv", self.q_dim + 2 * self.kv_dim, torch.float32)
+            self.qkv.store_codes(codes, scales, qkv, ctx.rows)
+            self._rotate_and_attend(ctx, call, qkv, residual)
+            return True
         inner = self.qkv.weight.shape[1]
         # (rows wider than a segment of K: only the kernel with a workgroup per half head takes them)
         takes_width = inner <= 2048 or ops.qkv_rope_gemm_ok(ctx.rows, self.head_dim, inner, self.heads + 2 * self.kv_heads)
@@ -288,11 +297,7 @@ class Attention(Mixer):
         if not turned:
             self.qkv.store(ws, h, qkv, rows)
         if rt.bf16:
-            q = ws.buffer("q_rot", self.q_dim, torch.bfloat16)
-            ops.rope_kvwrite(qkv, q, ctx.positions, ctx.row_seq, table, self.cos, self.sin,
-                             call.k_cache, call.v_cache, rows, self.heads, self.kv_heads, self.head_dim,
-                             ws.page_size, call.writes_cache)
-            self._attend(ctx, call, q, residual)
+            self._rotate_and_attend(ctx, call, qkv, residual)
         else:
             if not turned:
                 ops.rope_kvwrite(qkv, None, ctx.positions, ctx.row_seq, table, self.cos, self.sin,
@@ -301,6 +306,13 @@ class Attention(Mixer):
             out = ws.buffer("attn_out", self.q_dim, torch.float32)
             attend_f32(ctx, call, qkv, out, self.heads, self.kv_heads, self.head_dim, window, self.scale)
             self.o.add_into(ws, out, residual, rows)
+
+    def _rotate_and_attend(self, ctx, call, qkv, residual) -> None:
+        """The 32-bit q|k|v rows rotated, rounded and written into the cache, then attention."""
+        q = ctx.ws.buffer("q_rot", self.q_dim, torch.bfloat16)
+        ops.rope_kvwrite(qkv, q, ctx.positions, ctx.row_seq, ctx.block_tables[call.group], self.cos, self.sin, call.k_cache, call.v_cache,
+                         ctx.rows, self.heads, self.kv_heads, self.head_dim, ctx.ws.page_size, call.writes_cache)
+        self._attend(ctx, call, q, residual)
 
     def _attend(self, ctx, call, q, residual) -> None:
         """bfloat16 attention over the cache for rotated queries ``q``, then the output projection."""

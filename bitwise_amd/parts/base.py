@@ -25,10 +25,12 @@ class TensorSpec:
     weight in (0, 1)), "bias" (N(0, 1): gate biases, sinks), "small_bias" (N(0, 0.1)), "conv" (taps of a short convolution,
     N(0, 0.5)), "router" (N(0, 0.3)), "gate_matrix" (N(0, 1/in): square matrices in front of a sigmoid) or "int" (integer
     table, kept as int32).  ``below`` (integer tables): the entries lie in 0 .. below - 1 and those of a row differ.
+    ``block_scaled``: the part also takes the matrix in 8 bits, codes with a scale for each block (weights.block_scaled).
     """
     shape: Tuple[int, ...]
     kind: str = "linear"
     below: int = 0
+    block_scaled: bool = False
 
 
 @dataclass

@@ -10,6 +10,7 @@ from typing import Dict, Optional
 import torch
 
 from ..csrc import ops
+from ..weights.block_scaled import stacked
 from .base import FeedForward, TensorSpec, register_feed_forward
 from .linear import Linear
 
@@ -34,17 +35,22 @@ class SwiGLU(FeedForward):
 
     def tensors(self) -> Dict[str, TensorSpec]:
         return {
-            self.names[0]: TensorSpec((self.inter, self.width)),
-            self.names[1]: TensorSpec((self.inter, self.width)),
-            self.names[2]: TensorSpec((self.width, self.inter)),
+            self.names[0]: TensorSpec((self.inter, self.width), block_scaled=True),
+            self.names[1]: TensorSpec((self.inter, self.width), block_scaled=True),
+            self.names[2]: TensorSpec((self.width, self.inter), block_scaled=True),
         }
 
     def bind(self, tensors) -> None:
         g, u = tensors[self.names[0]], tensors[self.names[1]]
         if g.dtype != u.dtype:
             raise ValueError("gate and up projections must be stored in one dtype to be stacked")
-        self.gate_up = Linear(torch.cat([g, u], dim=0), self.rt)
+        self.gate_up = Linear(stacked([g, u]), self.rt)
         self.down = Linear(tensors[self.names[2]], self.rt)
+
+    @property
+    def in_codes(self) -> bool:
+        """All three matrices are in 8 bits (and run so): so are the rows between the products."""
+        return self.gate_up.fp8 and self.down.fp8
 
     def weight_bytes(self) -> int:
         return self.gate_up.nbytes() + self.down.nbytes()
@@ -53,6 +59,12 @@ class SwiGLU(FeedForward):
         """Decode steps of few rows: norm, the stacked product and SwiGLU are one kernel."""
         from .norm import RMSNorm
         rt, ws = self.rt, ctx.ws
+        if self.in_codes and type(norm) is RMSNorm:
+            # (any number of rows: the normed rows are in 8 bits at once, whatever step they are in)
+            codes, scales = self.gate_up.codes(ws)
+            ops.norm_add_norm(x, None, norm.weight, codes, ctx.rows, norm.eps, scales=scales)
+            self._from_codes(ctx, codes, scales, residual)
+            return True
         if not (rt.bf16 and isinstance(norm, RMSNorm) and self.gate_up.mfma and self.down.mfma
                 and ops.can_fuse_norm(ctx.rows, self.gate_up.weight, x, columns=32, stacked=2)):
             return False
@@ -61,9 +73,19 @@ class SwiGLU(FeedForward):
         self.down.add_into(ws, act, residual, ctx.rows)
         return True
 
+    def _from_codes(self, ctx, codes, scales, residual) -> None:
+        """The feed-forward of rows in 8 bits: gate, up and SwiGLU leave rows in 8 bits again."""
+        ws, rows = ctx.ws, ctx.rows
+        act, act_scales = ws.buffer("mlp_codes", ops.fp8_width(self.inter), ops.FP8), ws.buffer(
+            "mlp_codes_scales", ws.max_rows, torch.float32, rows=ops.fp8_width(self.inter) // ops.FP8_BLOCK)
+        self.gate_up.swiglu_codes(ws, codes, scales, act, act_scales, rows)
+        self.down.store_codes(act, act_scales, residual, rows, residual=residual)
+
     def forward(self, ctx, h, residual) -> None:
         rt, ws, rows = self.rt, ctx.ws, ctx.rows
-        if self.gate_up.mfma:
+        if self.in_codes:
+            self._from_codes(ctx, *self.gate_up._quantized(ws, h, rows), residual)
+        elif self.gate_up.mfma:
             act = ws.buffer("mlp_h", self.inter, torch.bfloat16)
             ops.gemm_bf16(h, self.gate_up.weight, act, rows, ops.EPI_SWIGLU_BF16)   # SwiGLU in the epilogue
         else:

@@ -3,7 +3,8 @@ seeded random weights written as a model folder.
 
 Dtype policy (the reference's converter, tools/convert.py:85-92, keeps BF16 and F32
 bytes and widens F16 to F32): bfloat16 stays bfloat16, a tensor stored in 32-bit stays
-32-bit, float16 is widened to float32, integer tables become int32.  Names are the
+32-bit, float16 is widened to float32, integer tables become int32; a matrix in 8 bits (e4m3 codes
+beside a tensor of scales) stays in 8 bits where the part that owns it takes it so.  Names are the
 checkpoint's own (src/model.cpp:136-171); nothing is renamed.
 """
 
@@ -17,7 +18,7 @@ from typing import Dict, Iterator, Mapping, Sequence, Tuple
 import torch
 
 from ..parts.base import TensorSpec
-from . import safetensors_io
+from . import block_scaled, safetensors_io
 
 
 class WeightError(ValueError):
@@ -36,7 +37,9 @@ def check_and_convert(specs: Mapping[str, TensorSpec], found: Mapping[str, torch
     over with an ``UnusedTensorWarning``).  Any other tensor the model has no use for is an error."""
     missing = [n for n in specs if n not in found]
     ignored = tuple(ignored_suffixes)
-    extra = [n for n in found if n not in specs and not (ignored and n.endswith(ignored))]
+    # (a matrix in 8 bits brings its scales under a name of their own)
+    scales = {n + block_scaled.SCALE_SUFFIX for n in specs if n in found and found[n].dtype == block_scaled.DTYPE}
+    extra = [n for n in found if n not in specs and n not in scales and not (ignored and n.endswith(ignored))]
     unexpected = [n for n in extra if n not in unused]
     tolerated = [n for n in extra if n in unused]
     wrong = []
@@ -66,6 +69,18 @@ def check_and_convert(specs: Mapping[str, TensorSpec], found: Mapping[str, torch
             out[name] = t
         elif t.dtype == torch.float16:
             out[name] = t.to(torch.float32)
+        elif t.dtype == block_scaled.DTYPE and spec.block_scaled:
+            s = found.get(name + block_scaled.SCALE_SUFFIX)
+            want = (block_scaled.blocks(spec.shape[0]), block_scaled.blocks(spec.shape[1]))
+            if s is None:
+                missing.append(name + block_scaled.SCALE_SUFFIX)
+            elif tuple(s.shape) != want or s.dtype not in (torch.float32, torch.bfloat16):
+                wrong.append(f"{name}{block_scaled.SCALE_SUFFIX}: stored {tuple(s.shape)} {s.dtype}, a floating scale for each block of "
+                             f"{block_scaled.BLOCK} x {block_scaled.BLOCK} is needed, {want}")
+            elif not bool(torch.isfinite(s).all()):
+                wrong.append(f"{name}{block_scaled.SCALE_SUFFIX}: scales that are no finite numbers")
+            else:
+                out[name] = block_scaled.BlockScaled([(t, s.float())], spec.shape[1])
         else:
             wrong.append(f"{name}: unsupported dtype {t.dtype}")
     if missing or unexpected or wrong:
@@ -124,6 +139,19 @@ def random_table(spec: TensorSpec, generator: torch.Generator, device="cpu") -> 
     return order[..., :n].to(torch.int32).contiguous()
 
 
+def stored_as(name: str, spec: TensorSpec, values: torch.Tensor, dtype: torch.dtype) -> Iterator[Tuple[str, torch.Tensor]]:
+    """The tensor or tensors that hold these values in a dtype.  8 bits: codes and scales where the part takes them, bfloat16
+    elsewhere."""
+    if dtype != block_scaled.DTYPE:
+        yield name, values.to(dtype)
+    elif spec.block_scaled:
+        codes, scales = block_scaled.quantize(values)
+        yield name, codes
+        yield name + block_scaled.SCALE_SUFFIX, scales
+    else:
+        yield name, values.to(torch.bfloat16)
+
+
 def random_tensors(specs: Mapping[str, TensorSpec], seed: int, sigma: float = 0.02,
                    dtype: torch.dtype = torch.bfloat16) -> Iterator[Tuple[str, torch.Tensor]]:
     """Seeded random weights, one tensor after the other in the order of ``specs``.
@@ -131,7 +159,8 @@ def random_tensors(specs: Mapping[str, TensorSpec], seed: int, sigma: float = 0.
     All draws come from one ``torch.Generator`` (CPU, ``manual_seed(seed)``) as float32
     standard normals in tensor order: linear and embedding weights are ``sigma * z``,
     norm weights ``1 + 0.1 * z``, integer tables as ``random_table`` draws them.  Values are then
-    rounded to ``dtype`` (round to nearest even for bfloat16).
+    rounded to ``dtype`` (round to nearest even for bfloat16; float8_e4m3fn: matrices of parts that take them so in 8 bits, the
+    rest in bfloat16).
     """
     g = torch.Generator(device="cpu")
     g.manual_seed(int(seed))
@@ -140,7 +169,7 @@ def random_tensors(specs: Mapping[str, TensorSpec], seed: int, sigma: float = 0.
             yield name, random_table(spec, g)
             continue
         z = torch.randn(spec.shape, generator=g, dtype=torch.float32)
-        yield name, shape_values(spec.kind, z, sigma).to(dtype)
+        yield from stored_as(name, spec, shape_values(spec.kind, z, sigma), dtype)
 
 
 def write_model_folder(folder: str | Path, config: Mapping[str, object], specs: Mapping[str, TensorSpec],

@@ -16,8 +16,8 @@ from typing import Dict, Iterable, Tuple
 import numpy as np
 import torch
 
-_NP_OF = {"F32": np.float32, "F16": np.float16, "BF16": np.uint16, "I32": np.int32, "I64": np.int64}
-_TORCH_TAG = {torch.float32: "F32", torch.float16: "F16", torch.bfloat16: "BF16",
+_NP_OF = {"F32": np.float32, "F16": np.float16, "BF16": np.uint16, "F8_E4M3": np.uint8, "I32": np.int32, "I64": np.int64}
+_TORCH_TAG = {torch.float32: "F32", torch.float16: "F16", torch.bfloat16: "BF16", torch.float8_e4m3fn: "F8_E4M3",
               torch.int32: "I32", torch.int64: "I64"}
 
 
@@ -43,7 +43,7 @@ def read_header(path: Path) -> Tuple[Dict[str, dict], int]:
 
 
 def read_file(path: str | Path) -> Dict[str, torch.Tensor]:
-    """All tensors of one file as CPU tensors viewing the memory map (BF16 as bfloat16)."""
+    """All tensors of one file as CPU tensors viewing the memory map (BF16 as bfloat16, F8_E4M3 as float8_e4m3fn)."""
     path = Path(path)
     header, base = read_header(path)
     data = np.memmap(path, dtype=np.uint8, mode="r")
@@ -67,6 +67,8 @@ def read_file(path: str | Path) -> Dict[str, torch.Tensor]:
         t = torch.from_numpy(arr)
         if tag == "BF16":
             t = t.view(torch.int16).view(torch.bfloat16)
+        elif tag == "F8_E4M3":
+            t = t.view(torch.float8_e4m3fn)
         out[name] = t
     spans.sort()
     for (_, e0, n0), (s1, _, n1) in zip(spans, spans[1:]):
@@ -97,7 +99,8 @@ def write_file(path: str | Path, tensors: Iterable[Tuple[str, torch.Tensor]]) ->
         if t.dtype not in _TORCH_TAG:
             raise SafetensorsError(f"cannot store dtype {t.dtype} of {name}")
         t = t.detach().contiguous().cpu()
-        raw = t.view(torch.int16).numpy().tobytes() if t.dtype == torch.bfloat16 else t.numpy().tobytes()
+        bits = {torch.bfloat16: torch.int16, torch.float8_e4m3fn: torch.uint8}.get(t.dtype)
+        raw = (t if bits is None else t.view(bits)).numpy().tobytes()
         header[name] = {"dtype": _TORCH_TAG[t.dtype], "shape": list(t.shape), "data_offsets": [offset, offset + len(raw)]}
         blobs.append(raw)
         offset += len(raw)
