@@ -2039,37 +2039,83 @@ def _need_rows(t: torch.Tensor, dtype, what: str) -> None:
         raise ValueError(f"{what} must be a matrix whose rows are contiguous")
 
 
-def _need_codes(codes: torch.Tensor, scales: torch.Tensor, rows: int, width: Optional[int], what: str) -> int:
-    """Rows of codes and their scales: [rows, whole blocks] e4m3 and [blocks, rows] float32, the rows of both contiguous;
-    returns the blocks."""
+# These calls are short where rows are few, and what Python does in front of a launch then counts as much as the launch: a
+# tensor's sizes and strides are asked for once, everything is looked at in one condition, and what is wrong is only worked out when
+# something is.  (A call with eleven checks as functions of their own took 8.5 us of the host's time, one so written 5.)
+
+def _matrix_arg(t: torch.Tensor, dtype, rows: int, width: int, device: int, what: str) -> Tuple[int, int]:
+    """A matrix [>= rows, width] on the device, rows contiguous and a stride apart: (pointer, stride; a single row's is its width)."""
+    if t.dtype is dtype and t.dim() == 2:
+        n, w = t.shape
+        ld, inner = t.stride()
+        if n >= rows and w == width and (inner == 1 or w == 1) and t.get_device() == device:
+            return t.data_ptr(), ld if rows > 1 else w
+    _need_rows(t, dtype, what)
+    if t.shape[0] < rows or t.shape[1] != width:
+        raise ValueError(f"{what} {tuple(t.shape)} does not fit {rows} rows of {width}")
+    raise ValueError(f"{what}: all tensors live on the current device")
+
+
+def _vector_arg(t: Optional[torch.Tensor], dim: int, device: int, what: str) -> Tuple[Optional[int], int]:
+    """A vector [dim], bfloat16 or float32, or None: (pointer, whether bfloat16)."""
+    if t is None:
+        return None, 0
+    if t.dim() != 1 or t.shape[0] != dim or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous vector of {dim} on the current device, on the GPU")
+    return t.data_ptr(), _is_bf16(t, what)
+
+
+def _codes_arg(codes: torch.Tensor, scales: torch.Tensor, rows: int, width: Optional[int], device: int, what: str) -> Tuple[int, int, int, int, int]:
+    """Rows of codes [>= rows, whole blocks] e4m3 and their scales [blocks, >= rows] float32, the rows of both contiguous:
+    (pointer, stride, scales' pointer, scales' stride from block to block, blocks)."""
+    if codes.dtype is FP8 and scales.dtype is torch.float32 and codes.dim() == 2 and scales.dim() == 2:
+        n, k = codes.shape
+        blocks, r = scales.shape
+        ld, inner = codes.stride()
+        lb, one = scales.stride()
+        at = codes.data_ptr()
+        if (n >= rows and r >= rows and k == blocks * FP8_BLOCK and k > 0 and inner == 1 and (one == 1 or r == 1) and at % 16 == 0
+                and (ld % 16 == 0 or rows <= 1) and (width is None or k - FP8_BLOCK < width <= k)
+                and codes.get_device() == device and scales.get_device() == device):
+            return at, ld if rows > 1 else k, scales.data_ptr(), lb if blocks > 1 else r, blocks
     _need_rows(codes, FP8, f"{what}: codes")
     _need_rows(scales, torch.float32, f"{what}: scales")
     if width is not None and codes.shape[1] != fp8_width(width):
         raise ValueError(f"{what}: codes of rows of {width} elements are {fp8_width(width)} wide, got {codes.shape[1]}")
     if codes.shape[1] % FP8_BLOCK or codes.shape[1] == 0:
         raise ValueError(f"{what}: rows of codes are whole blocks of {FP8_BLOCK}, got {codes.shape[1]}")
-    blocks = codes.shape[1] // FP8_BLOCK
-    if codes.shape[0] < rows or scales.shape[0] != blocks or scales.shape[1] < rows:
+    if codes.shape[0] < rows or scales.shape[0] != codes.shape[1] // FP8_BLOCK or scales.shape[1] < rows:
         raise ValueError(f"{what}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} (blocks by rows) do not fit {rows} rows")
     if codes.data_ptr() % 16 or (rows > 1 and codes.stride(0) % 16):
         raise ValueError(f"{what}: rows of codes start at multiples of 16 bytes")
-    return blocks
+    raise ValueError(f"{what}: all tensors live on the current device")
 
 
-def _ld(t: Optional[torch.Tensor], rows: int) -> int:
-    """The stride of a matrix's rows (of a single row its width: the tensor's own says nothing)."""
-    return 0 if t is None else t.stride(0) if rows > 1 else t.shape[1]
-
-
-def _lb(scales: Optional[torch.Tensor]) -> int:
-    """The stride of rows' scales from block to block."""
-    return 0 if scales is None else _ld(scales, scales.shape[0])
-
-
-def _same_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1 or next(iter(devices)).index != torch.cuda.current_device():
+def _fp8_matrix_arg(w: torch.Tensor, w_scales: torch.Tensor, halves: int, blocks: int, device: int, what: str) -> Tuple[int, int, int]:
+    """A matrix [halves * N, blocks * 128] of codes with its scales: (pointer, scales' pointer, N)."""
+    if w.dtype is FP8 and w_scales.dtype is torch.float32 and w.dim() == 2 and w_scales.dim() == 2:
+        n, k = w.shape
+        nb, kb = w_scales.shape
+        if (n > 0 and n % halves == 0 and k == blocks * FP8_BLOCK and kb == blocks and nb == halves * (-(-(n // halves) // FP8_BLOCK))
+                and w.is_contiguous() and w_scales.is_contiguous() and w.get_device() == device and w_scales.get_device() == device):
+            return w.data_ptr(), w_scales.data_ptr(), n // halves
+    _need(w, FP8, f"{what}: weight")
+    _need(w_scales, torch.float32, f"{what}: weight scales")
+    if w.dim() != 2 or w.shape[0] % halves or w.shape[0] == 0:
+        raise ValueError(f"{what}: weight must be a matrix" + (" of gate rows, then as many up rows" if halves == 2 else ""))
+    if w.get_device() != device or w_scales.get_device() != device:
         raise ValueError(f"{what}: all tensors live on the current device")
+    raise ValueError(f"{what}: weight {tuple(w.shape)} with scales {tuple(w_scales.shape)} does not fit rows of {blocks} blocks of {FP8_BLOCK}")
+
+
+def _device_of(t: torch.Tensor, what: str) -> int:
+    """The device of a call's first tensor, which has to be the current one (the stream is its)."""
+    device = t.get_device()
+    if device < 0:
+        raise ValueError(f"{what} must live on the GPU (there is no CPU path)")
+    if device != (_raw_device() if _raw_device is not None else torch.cuda.current_device()):
+        raise ValueError(f"{what}: all tensors live on the current device")
+    return device
 
 
 def quantize_fp8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, rows: int) -> None:
@@ -2079,15 +2125,15 @@ def quantize_fp8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, row
 
     all in 32 bits, the codes rounded to nearest even.  ``codes`` [>= rows, fp8_width(K)] gets zeros behind the rows' end;
     ``scales`` [fp8_width(K) / 128, >= rows].  A block that holds an infinity or NaN stands for NaN throughout."""
-    if x.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"quantize_fp8: x must be bfloat16 or float32, got {x.dtype}")
-    _need_rows(x, x.dtype, "quantize_fp8: x")
-    _need_codes(codes, scales, rows, x.shape[1], "quantize_fp8")
-    if x.shape[0] < rows:
-        raise ValueError("quantize_fp8: x is shorter than the rows")
-    _same_device("quantize_fp8", x, codes, scales)
-    _check(_fn("bw_quantize_fp8")(x.data_ptr(), _is_bf16(x, "x"), _ld(x, rows), codes.data_ptr(), _ld(codes, rows), scales.data_ptr(), _lb(scales),
-                                  rows, x.shape[1], _stream()), "quantize_fp8")
+    dtype = x.dtype
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
+        raise ValueError(f"quantize_fp8: x must be bfloat16 or float32, got {dtype}")
+    if x.dim() != 2:
+        raise ValueError("quantize_fp8: x must be a matrix")
+    device, width = _device_of(x, "quantize_fp8: x"), x.shape[1]
+    xp, ldx = _matrix_arg(x, dtype, rows, width, device, "quantize_fp8: x")
+    cp, ldc, sp, lds, _ = _codes_arg(codes, scales, rows, width, device, "quantize_fp8")
+    _check(_fn("bw_quantize_fp8")(xp, dtype is torch.bfloat16, ldx, cp, ldc, sp, lds, rows, width, _stream()), "quantize_fp8")
 
 
 def norm_add_norm(x: torch.Tensor, y: Optional[torch.Tensor], weight: torch.Tensor, out: torch.Tensor, rows: int, eps: float,
@@ -2103,71 +2149,41 @@ def norm_add_norm(x: torch.Tensor, y: Optional[torch.Tensor], weight: torch.Tens
     float32 each.  ``stream`` (float32) may be x and is x if not given.  ``out`` is float32, bfloat16 (one rounding) or e4m3
     codes [rows, fp8_width(dim)] with ``scales`` as ``quantize_fp8`` of the 32-bit rows gives them.  y None: out = norm(x) *
     weight, and nothing else is given."""
-    _need_rows(x, torch.float32, "norm_add_norm: x")
-    dim = x.shape[1]
-
-    def vector(t, what):
-        if t is None:
-            return None, 0
-        if t.dim() != 1 or t.shape[0] != dim or not t.is_cuda or not t.is_contiguous():
-            raise ValueError(f"norm_add_norm: {what} must be a contiguous vector of {dim} on the GPU")
-        return t.data_ptr(), _is_bf16(t, what)
-
-    def matrix(t, what):
-        _need_rows(t, t.dtype, f"norm_add_norm: {what}")
-        if t.shape[0] < rows or t.shape[1] != dim:
-            raise ValueError(f"norm_add_norm: {what} {tuple(t.shape)} does not fit {rows} rows of {dim}")
-        return t.data_ptr(), _is_bf16(t, what), _ld(t, rows)
-
-    if x.shape[0] < rows:
-        raise ValueError("norm_add_norm: x is shorter than the rows")
-    scale_vec = scale if isinstance(scale, torch.Tensor) else None
-    if y is None and not (post_weight is None and gate is None and stream is None and scale_vec is None and scale == 1.0):
-        raise ValueError("norm_add_norm: without a sublayer's output there is nothing to norm, gate, scale or add")
-    if stream is None and y is not None:
-        stream = x
-    if stream is not None:
-        _need_rows(stream, torch.float32, "norm_add_norm: stream")
-        if stream.shape[0] < rows or stream.shape[1] != dim:
-            raise ValueError(f"norm_add_norm: stream {tuple(stream.shape)} does not fit {rows} rows of {dim}")
-    if (scales is not None) != (out.dtype == FP8):
+    if x.dim() != 2:
+        raise ValueError("norm_add_norm: x must be a matrix")
+    device, dim = _device_of(x, "norm_add_norm: x"), x.shape[1]
+    xp, ldx = _matrix_arg(x, torch.float32, rows, dim, device, "norm_add_norm: x")
+    vector = isinstance(scale, torch.Tensor)
+    yp = yb = ldy = gp = gb = ldg = tp = ldt = 0
+    if y is None:
+        if post_weight is not None or gate is not None or stream is not None or vector or scale != 1.0:
+            raise ValueError("norm_add_norm: without a sublayer's output there is nothing to norm, gate, scale or add")
+    else:
+        yb = _is_bf16(y, "norm_add_norm: y")
+        yp, ldy = _matrix_arg(y, y.dtype, rows, dim, device, "norm_add_norm: y")
+        tp, ldt = (xp, ldx) if stream is None else _matrix_arg(stream, torch.float32, rows, dim, device, "norm_add_norm: stream")
+    if gate is not None:
+        if gate.dim() == 2:
+            gb = _is_bf16(gate, "norm_add_norm: gate")
+            gp, ldg = _matrix_arg(gate, gate.dtype, rows, dim, device, "norm_add_norm: gate")
+            if ldg == 0:
+                raise ValueError("norm_add_norm: a gate for all rows is a vector")
+        else:
+            gp, gb = _vector_arg(gate, dim, device, "norm_add_norm: gate")
+    cp, lds = 0, 0
+    if (scales is not None) != (out.dtype is FP8):
         raise ValueError("norm_add_norm: codes come with scales, other rows without")
-    if out.dtype == FP8:
-        _need_codes(out, scales, rows, dim, "norm_add_norm")
-        kind, ldo = 2, _ld(out, rows)
+    if scales is not None:
+        op, ldo, cp, lds, _ = _codes_arg(out, scales, rows, dim, device, "norm_add_norm")
+        kind = 2
     else:
-        _, kind, ldo = matrix(out, "out")
-    yp, yb, ldy = (None, 0, 0) if y is None else matrix(y, "y")
-    if gate is None:
-        gp, gb, ldg = None, 0, 0
-    elif gate.dim() == 2:
-        gp, gb, ldg = matrix(gate, "gate")
-        if ldg == 0:
-            raise ValueError("norm_add_norm: a gate for all rows is a vector")
-    else:
-        gp, gb = vector(gate, "gate")
-        ldg = 0
-    pp, pb = vector(post_weight, "post_weight")
-    sp, sb = vector(scale_vec, "scale")
-    wp, wb = vector(weight, "weight")
-    _same_device("norm_add_norm", x, y, weight, out, post_weight, gate, scale_vec, stream, scales)
-    _check(_fn("bw_norm_add_norm")(x.data_ptr(), _ld(x, rows), yp, yb, ldy, pp, pb, float(eps if post_eps is None else post_eps), gp, gb, ldg,
-                                   int(bool(gate_sigmoid)), sp, sb, 0.0 if scale_vec is not None else float(scale),
-                                   None if stream is None else stream.data_ptr(), _ld(stream, rows), wp, wb, float(eps),
-                                   out.data_ptr(), kind, ldo, None if scales is None else scales.data_ptr(), _lb(scales),
-                                   rows, dim, _stream()), "norm_add_norm")
-
-
-def _need_fp8_matrix(w: torch.Tensor, w_scales: torch.Tensor, halves: int, blocks: int, what: str) -> int:
-    """A matrix [halves * N, K] of codes with its scales; returns N."""
-    _need(w, FP8, f"{what}: weight")
-    _need(w_scales, torch.float32, f"{what}: weight scales")
-    if w.dim() != 2 or w.shape[0] % halves or w.shape[0] == 0:
-        raise ValueError(f"{what}: weight must be a matrix" + (" of gate rows, then as many up rows" if halves == 2 else ""))
-    n = w.shape[0] // halves
-    if w.shape[1] != blocks * FP8_BLOCK or tuple(w_scales.shape) != (halves * (-(-n // FP8_BLOCK)), blocks):
-        raise ValueError(f"{what}: weight {tuple(w.shape)} with scales {tuple(w_scales.shape)} does not fit rows of {blocks} blocks of {FP8_BLOCK}")
-    return n
+        kind = _is_bf16(out, "norm_add_norm: out")
+        op, ldo = _matrix_arg(out, out.dtype, rows, dim, device, "norm_add_norm: out")
+    pp, pb = _vector_arg(post_weight, dim, device, "norm_add_norm: post_weight")
+    vp, vb = _vector_arg(scale if vector else None, dim, device, "norm_add_norm: scale")
+    wp, wb = _vector_arg(weight, dim, device, "norm_add_norm: weight")
+    _check(_fn("bw_norm_add_norm")(xp, ldx, yp, yb, ldy, pp, pb, eps if post_eps is None else post_eps, gp, gb, ldg, bool(gate_sigmoid), vp, vb,
+                                   0.0 if vector else scale, tp, ldt, wp, wb, eps, op, kind, ldo, cp, lds, rows, dim, _stream()), "norm_add_norm")
 
 
 def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, rows: int,
@@ -2177,20 +2193,17 @@ def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales:
     block.  Each block's products are summed in 32 bits, the blocks' sums times their two scales are added up in 32 bits, k
     ascending: a row's bits do not depend on the rows beside it.  ``out`` is float32 or bfloat16 (one rounding), its rows a stride
     apart; ``residual`` (float32, with a float32 ``out``, which it may be) is added last."""
-    blocks = _need_codes(x, x_scales, rows, None, "gemm_fp8")
-    n = _need_fp8_matrix(w, w_scales, 1, blocks, "gemm_fp8")
-    bf16 = _is_bf16(out, "out")
-    _need_rows(out, out.dtype, "gemm_fp8: out")
-    if out.shape[0] < rows or out.shape[1] != n:
-        raise ValueError(f"gemm_fp8: out {tuple(out.shape)} does not fit {rows} rows of {n}")
+    device = _device_of(x, "gemm_fp8: x")
+    xp, ldx, sp, lds, blocks = _codes_arg(x, x_scales, rows, None, device, "gemm_fp8")
+    wp, wsp, n = _fp8_matrix_arg(w, w_scales, 1, blocks, device, "gemm_fp8")
+    bf16 = _is_bf16(out, "gemm_fp8: out")
+    op, ldo = _matrix_arg(out, out.dtype, rows, n, device, "gemm_fp8: out")
+    rp = ldr = 0
     if residual is not None:
-        _need_rows(residual, torch.float32, "gemm_fp8: residual")
-        if bf16 or residual.shape[0] < rows or residual.shape[1] != n:
-            raise ValueError("gemm_fp8: a residual has out's width, and out is 32-bit then")
-    _same_device("gemm_fp8", x, x_scales, w, w_scales, out, residual)
-    _check(_fn("bw_gemm_fp8")(x.data_ptr(), _ld(x, rows), x_scales.data_ptr(), _lb(x_scales), w.data_ptr(), w_scales.data_ptr(),
-                              None if residual is None else residual.data_ptr(), _ld(residual, rows),
-                              out.data_ptr(), _ld(out, rows), bf16, rows, n, x.shape[1], _stream()), "gemm_fp8")
+        if bf16:
+            raise ValueError("gemm_fp8: what is added to a residual stays 32-bit")
+        rp, ldr = _matrix_arg(residual, torch.float32, rows, n, device, "gemm_fp8: residual")
+    _check(_fn("bw_gemm_fp8")(xp, ldx, sp, lds, wp, wsp, rp, ldr, op, ldo, bf16, rows, n, blocks * FP8_BLOCK, _stream()), "gemm_fp8")
 
 
 def gemm_fp8_swiglu(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, codes: torch.Tensor,
@@ -2199,21 +2212,16 @@ def gemm_fp8_swiglu(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_
     ready for the product with its down projection.  ``w`` [2N, K] holds the gate rows, then the up rows, each half with scale
     blocks of its own: ``w_scales`` [2 ceil(N / 128), K / 128].  More than 64 rows: one launch, whose epilogue does it all; up to 64
     rows need ``sums`` (float32 [>= rows, N]), where silu(g) * u lies between two launches.  The bits are the same either way."""
-    blocks = _need_codes(x, x_scales, rows, None, "gemm_fp8_swiglu")
-    n = _need_fp8_matrix(w, w_scales, 2, blocks, "gemm_fp8_swiglu")
-    _need_codes(codes, scales, rows, n, "gemm_fp8_swiglu")
+    device = _device_of(x, "gemm_fp8_swiglu: x")
+    xp, ldx, sp, lds, blocks = _codes_arg(x, x_scales, rows, None, device, "gemm_fp8_swiglu")
+    wp, wsp, n = _fp8_matrix_arg(w, w_scales, 2, blocks, device, "gemm_fp8_swiglu")
+    cp, ldc, osp, ldos, _ = _codes_arg(codes, scales, rows, n, device, "gemm_fp8_swiglu")
+    up = ldu = 0
     if rows <= FP8_SUMS_ROWS:
         if sums is None:
             raise ValueError(f"gemm_fp8_swiglu: up to {FP8_SUMS_ROWS} rows need a buffer for their sums")
-        _need_rows(sums, torch.float32, "gemm_fp8_swiglu: sums")
-        if sums.shape[0] < rows or sums.shape[1] != n:
-            raise ValueError(f"gemm_fp8_swiglu: sums {tuple(sums.shape)} do not fit {rows} rows of {n}")
-    else:
-        sums = None
-    _same_device("gemm_fp8_swiglu", x, x_scales, w, w_scales, codes, scales, sums)
-    _check(_fn("bw_gemm_fp8_swiglu")(x.data_ptr(), _ld(x, rows), x_scales.data_ptr(), _lb(x_scales), w.data_ptr(), w_scales.data_ptr(),
-                                     None if sums is None else sums.data_ptr(), _ld(sums, rows), codes.data_ptr(),
-                                     _ld(codes, rows), scales.data_ptr(), _lb(scales), rows, n, x.shape[1], _stream()), "gemm_fp8_swiglu")
+        up, ldu = _matrix_arg(sums, torch.float32, rows, n, device, "gemm_fp8_swiglu: sums")
+    _check(_fn("bw_gemm_fp8_swiglu")(xp, ldx, sp, lds, wp, wsp, up, ldu, cp, ldc, osp, ldos, rows, n, blocks * FP8_BLOCK, _stream()), "gemm_fp8_swiglu")
 
 
 # ------------------------------------------------------------------------------ sampling
