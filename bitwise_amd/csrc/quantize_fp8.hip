@@ -126,60 +126,42 @@ __device__ __forceinline__ float row_inverse(float acc, float* part, int dim, fl
   acc = wave_sum(acc);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = acc;
   __syncthreads();
-  return 1.0f / sqrtf((((part[0] + part[1]) + part[2]) + part[3]) / (float)dim + eps);
+  float total = part[0];
+  for (int v = 1; v < (int)(blockDim.x >> 6); ++v) total += part[v];
+  return 1.0f / sqrtf(total / (float)dim + eps);
 }
 
-// A workgroup a row, thread t the eights t, t + 256, ...  J > 0: the row stays in registers, all loads are asked for first, and
-// everything is read once.  J = 0: rows of any width, in passes (the stream is read back by the threads that wrote it).
-template <int J, bool VEC>
-__global__ __launch_bounds__(256) void norm_add_norm_kernel(NormAddNormArgs a) {
-  __shared__ float part[2][4];
+// A workgroup a row.  WHOLE: as many threads as the row has eights of elements: all loads are asked for first, everything is read
+// once.  Otherwise (rows of more than 8,192) thread t has the eights t, t + 1024, ... in passes, and reads the stream back that it
+// wrote.
+template <bool WHOLE, bool VEC>
+__global__ __launch_bounds__(1024) void norm_add_norm_kernel(NormAddNormArgs a) {
+  __shared__ float part[2][16];
   const size_t row = blockIdx.x;
   const int whole = a.out_kind == OUT_FP8 ? (a.dim + BW_FP8_BLOCK - 1) / BW_FP8_BLOCK * BW_FP8_BLOCK : a.dim;
   const Raw8 none = {(u32x4){0u, 0u, 0u, 0u}, (u32x4){0u, 0u, 0u, 0u}};
-  if constexpr (J > 0) {
-    Raw8 rx[J], ry[J], rg[J], rp[J], rs[J], rw[J];
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int e = 8 * ((int)threadIdx.x + 256 * j);
-      ry[j] = a.y != nullptr ? load_raw8<VEC>(a.y, a.y_bf16, row * a.ldy, e, a.dim) : none;
-      rx[j] = load_raw8<VEC>(a.x, 0, row * a.ldx, e, a.dim);
-      rg[j] = a.gate != nullptr ? load_raw8<VEC>(a.gate, a.gate_bf16, row * a.ldg, e, a.dim) : none;
-      rp[j] = a.post_weight != nullptr ? load_raw8<VEC>(a.post_weight, a.post_bf16, 0, e, a.dim) : none;
-      rs[j] = a.scale_vec != nullptr ? load_raw8<VEC>(a.scale_vec, a.scale_bf16, 0, e, a.dim) : none;
-      rw[j] = load_raw8<VEC>(a.weight, a.weight_bf16, 0, e, a.dim);
+  if constexpr (WHOLE) {
+    const int e = 8 * (int)threadIdx.x;
+    const Raw8 ry = a.y != nullptr ? load_raw8<VEC>(a.y, a.y_bf16, row * a.ldy, e, a.dim) : none;
+    const Raw8 rx = load_raw8<VEC>(a.x, 0, row * a.ldx, e, a.dim);
+    const Raw8 rg = a.gate != nullptr ? load_raw8<VEC>(a.gate, a.gate_bf16, row * a.ldg, e, a.dim) : none;
+    const Raw8 rp = a.post_weight != nullptr ? load_raw8<VEC>(a.post_weight, a.post_bf16, 0, e, a.dim) : none;
+    const Raw8 rs = a.scale_vec != nullptr ? load_raw8<VEC>(a.scale_vec, a.scale_bf16, 0, e, a.dim) : none;
+    const Raw8 rw = load_raw8<VEC>(a.weight, a.weight_bf16, 0, e, a.dim);
+    float x[8];
+    raw8_floats<VEC>(rx, 0, x);
+    if (a.y != nullptr) {
+      float y[8], inv = 0.0f;
+      raw8_floats<VEC>(ry, a.y_bf16, y);
+      if (a.post_weight != nullptr) inv = row_inverse(sumsq8(y, 0.0f), part[0], a.dim, a.post_eps);
+      branch_step<VEC>(a, y, inv, rp, rg, rs, x);
+      store_stream<VEC>(a, row, e, x);
     }
-    float x[J][8];
-    float inv = 0.0f, acc = 0.0f;
-    if (a.post_weight != nullptr) {
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        float y[8];
-        raw8_floats<VEC>(ry[j], a.y_bf16, y);
-        acc = sumsq8(y, acc);
-      }
-      inv = row_inverse(acc, part[0], a.dim, a.post_eps);
-    }
-    acc = 0.0f;
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int e = 8 * ((int)threadIdx.x + 256 * j);
-      raw8_floats<VEC>(rx[j], 0, x[j]);
-      if (a.y != nullptr) {
-        float y[8];
-        raw8_floats<VEC>(ry[j], a.y_bf16, y);
-        branch_step<VEC>(a, y, inv, rp[j], rg[j], rs[j], x[j]);
-        store_stream<VEC>(a, row, e, x[j]);
-      }
-      acc = sumsq8(x[j], acc);
-    }
-    const float inv2 = row_inverse(acc, part[1], a.dim, a.eps);
-#pragma unroll
-    for (int j = 0; j < J; ++j) store_normed<VEC>(a, row, 8 * ((int)threadIdx.x + 256 * j), whole, x[j], inv2, rw[j]);
+    store_normed<VEC>(a, row, e, whole, x, row_inverse(sumsq8(x, 0.0f), part[1], a.dim, a.eps), rw);
   } else {
     float inv = 0.0f, acc = 0.0f;
     if (a.post_weight != nullptr) {
-      for (int e = 8 * (int)threadIdx.x; e < a.dim; e += 2048) {
+      for (int e = 8 * (int)threadIdx.x; e < a.dim; e += 8192) {
         float y[8];
         raw8_floats<VEC>(load_raw8<VEC>(a.y, a.y_bf16, row * a.ldy, e, a.dim), a.y_bf16, y);
         acc = sumsq8(y, acc);
@@ -187,7 +169,7 @@ __global__ __launch_bounds__(256) void norm_add_norm_kernel(NormAddNormArgs a) {
       inv = row_inverse(acc, part[0], a.dim, a.post_eps);
     }
     acc = 0.0f;
-    for (int e = 8 * (int)threadIdx.x; e < a.dim; e += 2048) {
+    for (int e = 8 * (int)threadIdx.x; e < a.dim; e += 8192) {
       float x[8];
       raw8_floats<VEC>(load_raw8<VEC>(a.x, 0, row * a.ldx, e, a.dim), 0, x);
       if (a.y != nullptr) {
@@ -202,7 +184,7 @@ __global__ __launch_bounds__(256) void norm_add_norm_kernel(NormAddNormArgs a) {
     }
     const float inv2 = row_inverse(acc, part[1], a.dim, a.eps);
     const float* from = a.y != nullptr ? a.stream + row * a.ldst : a.x + row * a.ldx;
-    for (int e = 8 * (int)threadIdx.x; e < ((whole + 127) & ~127); e += 2048) {      // (whole rows of 16 lanes)
+    for (int e = 8 * (int)threadIdx.x; e < ((whole + 127) & ~127); e += 8192) {      // (whole rows of 16 lanes)
       float x[8];
       raw8_floats<VEC>(load_raw8<VEC>(from, 0, 0, e, a.dim), 0, x);
       store_normed<VEC>(a, row, e, whole, x, inv2, load_raw8<VEC>(a.weight, a.weight_bf16, 0, e, a.dim));
@@ -246,16 +228,15 @@ extern "C" int bw_norm_add_norm(const float* x, int ldx, const void* y, int y_is
   const bool vec = dim % 8 == 0 && fits(x, 0, ldx) && fits(y, y_is_bf16, ldy) && fits(post_weight, post_is_bf16, 0) && fits(gate, gate_is_bf16, ldg) &&
                    fits(scale_vec, scale_is_bf16, 0) && fits(weight, weight_is_bf16, 0) && fits(y != nullptr ? stream_out : nullptr, 0, ldst) &&
                    (out_kind == OUT_FP8 || fits(out, out_kind == OUT_BF16, ldo));
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(256), 0, (hipStream_t)stream, a); };
-  if (vec) {
-    if (dim <= 2048) launch(norm_add_norm_kernel<1, true>);
-    else if (dim <= 4096) launch(norm_add_norm_kernel<2, true>);
-    else if (dim <= 6144) launch(norm_add_norm_kernel<3, true>);
-    else if (dim <= 8192) launch(norm_add_norm_kernel<4, true>);
-    else launch(norm_add_norm_kernel<0, true>);
+  // (whole waves; rows of codes end with whole blocks)
+  const int threads = dim > 8192 ? 1024 : (dim + 511) / 512 * 64;
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(threads), 0, (hipStream_t)stream, a); };
+  if (dim <= 8192) {
+    if (vec) launch(norm_add_norm_kernel<true, true>);
+    else launch(norm_add_norm_kernel<true, false>);
   } else {
-    if (dim <= 2048) launch(norm_add_norm_kernel<1, false>);
-    else launch(norm_add_norm_kernel<0, false>);
+    if (vec) launch(norm_add_norm_kernel<false, true>);
+    else launch(norm_add_norm_kernel<false, false>);
   }
   return BW_LAUNCH_CHECK();
 }
