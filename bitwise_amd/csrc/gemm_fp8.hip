@@ -32,6 +32,7 @@ struct Fp8Args {
   int ldx, ldxs, ldr, ldo, lds;
   int M, N, K;               // N: output columns (gated: half the matrix's rows); K: the padded inner size
   int m_tiles, n_tiles;
+  int vec_out;               // rows of out and residual can be taken 16 bytes at a time
 };
 
 // A block's 128 codes of 16 rows as the matrix instructions take them: lane (g, r) has row r's bytes 16 g and 64 + 16 g of the block
@@ -46,14 +47,15 @@ __device__ __forceinline__ uint32_t codes_to_bf16x2(uint32_t four, bool upper) {
                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, 1.0f, false));
 }
 
+__device__ __forceinline__ bf16x8 quarter_of(u32x4 half, int odd) {
+  const uint32_t a = half[2 * odd], b = half[2 * odd + 1];
+  return as_bf16x8((u32x4){codes_to_bf16x2(a, false), codes_to_bf16x2(a, true), codes_to_bf16x2(b, false), codes_to_bf16x2(b, true)});
+}
+
 __device__ __forceinline__ Frag frag_of(u32x4 lo, u32x4 hi) {
   Frag f;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const u32x4 v = t < 2 ? lo : hi;
-    const uint32_t a = v[2 * (t & 1)], b = v[2 * (t & 1) + 1];
-    f.t[t] = as_bf16x8((u32x4){codes_to_bf16x2(a, false), codes_to_bf16x2(a, true), codes_to_bf16x2(b, false), codes_to_bf16x2(b, true)});
-  }
+  for (int t = 0; t < 4; ++t) f.t[t] = quarter_of(t < 2 ? lo : hi, t & 1);
   return f;
 }
 
@@ -93,22 +95,24 @@ __device__ __forceinline__ void store_one(const Fp8Args& a, int m, int n, float 
 
 // ------------------------------------------------------------------------------ few rows
 
-// Up to 64 rows: a workgroup of NW waves a strip of 16 matrix rows (gated: 16 gate and 16 up rows).  In round t wave v
-// computes the sums of block t NW + v; they meet in LDS, where the threads that own the outputs walk them in order.
-template <int WM, int EPI, int NW, int D>
+// Up to 64 rows: a workgroup of NW waves a strip of CW matrix rows (gated: CW gate and CW up rows).  The blocks of K go round the
+// waves, D to a wave and pass, all asked for before any is waited for; their sums meet in LDS, where the threads that own the outputs
+// walk them in order.  CW = 8 halves the strip (lanes with r >= 8 ask for nothing): twice as many workgroups, for products with too
+// few columns to give every compute unit 16.
+template <int WM, int EPI, int NW, int D, int CW>
 __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
   constexpr int NB = EPI == SWIGLU_F32 ? 2 : 1;
-  constexpr int OWN = (WM * 256 + 64 * NW - 1) / (64 * NW);
-  __shared__ __attribute__((aligned(16))) float part[2][NW][NB][WM][256];
-  __shared__ float factor[2][NW][NB][WM * 16];
+  constexpr int PS = 16 * CW, OWNED = WM * PS, OWN = (OWNED + 64 * NW - 1) / (64 * NW), C = NW * D;
+  extern __shared__ __attribute__((aligned(16))) float part[];                  // [C][NB][WM][PS], then the factors
+  float* factor = part + C * NB * WM * PS;                                      // [C][NB][WM * 16]
   const int wave = wave_index(), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, KB = a.K / BW_FP8_BLOCK;
-  const int w_rows = min(16, a.N - n0);
+  const int n0 = blockIdx.x * CW, KB = a.K / BW_FP8_BLOCK;
+  const int w_rows = min(CW, a.N - n0);
   __amdgpu_buffer_rsrc_t rs_w[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) rs_w[b] = rows_of(a.w + ((size_t)b * a.N + n0) * a.K, (size_t)w_rows * a.K);
   const __amdgpu_buffer_rsrc_t rs_x = rows_of(a.x, (size_t)(a.M - 1) * a.ldx + a.K);
-  const int voff_w = r * a.K + 16 * g;
+  const int voff_w = r < CW ? r * a.K + 16 * g : OUTSIDE;
   int voff_x[WM], row_m[WM];
 #pragma unroll
   for (int i = 0; i < WM; ++i) {
@@ -121,8 +125,8 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
 
   u32x4 wq[D][NB][2], xq[D][WM][2];
   float sx[D][WM], sw[D][NB];
-  auto issue = [&](int d, int round) {
-    const int blk = min(round * NW + wave, KB - 1);            // (past the end: the last block again, whose sums nobody takes)
+  auto issue = [&](int d, int pass) {
+    const int blk = min((pass * D + d) * NW + wave, KB - 1);     // (past the end: the last block again, whose sums nobody takes)
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       wq[d][b][0] = __builtin_amdgcn_raw_buffer_load_b128(rs_w[b], voff_w, blk * BW_FP8_BLOCK, 0);
@@ -138,21 +142,21 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) sw[d][b] = ws_row[b][blk];
   };
-  const int rounds = (KB + NW - 1) / NW;
+  const int passes = (KB + C - 1) / C;
 #pragma unroll
-  for (int d = 0; d < D; ++d) issue(d, d);
+  for (int d = 0; d < D; ++d) issue(d, 0);
   __builtin_amdgcn_sched_barrier(0);
   float acc[NB][OWN];
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int o = 0; o < OWN; ++o) acc[b][o] = 0.0f;
-  for (int t0 = 0; t0 < rounds; t0 += D) {
+  for (int pass = 0; pass < passes; ++pass) {
+    if (pass > 0) lds_barrier();                                 // (the sums of the pass before have been walked)
 #pragma unroll
     for (int d = 0; d < D; ++d) {
-      const int t = t0 + d;
-      if (t < rounds) {                                          // (scalar)
-        const int buf = t & 1;
+      const int at = d * NW + wave;
+      if (pass * C + at < KB) {                                  // (scalar)
         Frag fw[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) fw[b] = frag_of(wq[d][b][0], wq[d][b][1]);
@@ -161,64 +165,73 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
           const Frag fx = frag_of(xq[d][i][0], xq[d][i][1]);
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
-            *reinterpret_cast<f32x4*>(&part[buf][wave][b][i][4 * lane]) = block_sums(fw[b], fx);
-            if (g == 0) factor[buf][wave][b][16 * i + r] = sx[d][i] * sw[d][b];
+            const f32x4 sums = block_sums(fw[b], fx);
+            if (CW == 16 || lane < 32) *reinterpret_cast<f32x4*>(part + ((at * NB + b) * WM + i) * PS + 4 * lane) = sums;
+            if (g == 0) factor[(at * NB + b) * (WM * 16) + 16 * i + r] = sx[d][i] * sw[d][b];
           }
         }
-        issue(d, t + D);
-        __builtin_amdgcn_sched_barrier(0);
-        lds_barrier();
-        const int here = min(NW, KB - t * NW);
+      }
+      if (pass + 1 < passes) issue(d, pass + 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    lds_barrier();
+    const int here = min(C, KB - pass * C);
 #pragma unroll
-        for (int o = 0; o < OWN; ++o) {
-          const int at = (int)threadIdx.x + o * 64 * NW;
-          if (at < WM * 256) {
-            const int i = at >> 8, m = 16 * i + ((at >> 2) & 15);
-            auto walk = [&](int v) {
+    for (int o = 0; o < OWN; ++o) {
+      const int e = (int)threadIdx.x + o * 64 * NW;
+      if (e < OWNED) {
+        const int m = 16 * (e / PS) + ((e >> 2) & 15);
+        auto walk = [&](int v) {
 #pragma unroll
-              for (int b = 0; b < NB; ++b) acc[b][o] = fmaf(factor[buf][v][b][m], part[buf][v][b][i][at & 255], acc[b][o]);
-            };
-            if (here == NW) {
-#pragma unroll
-              for (int v = 0; v < NW; ++v) walk(v);
-            } else {
-              for (int v = 0; v < here; ++v) walk(v);
-            }
-          }
+          for (int b = 0; b < NB; ++b) acc[b][o] = fmaf(factor[(v * NB + b) * (WM * 16) + m], part[(v * NB + b) * (WM * PS) + e], acc[b][o]);
+        };
+        if (here == C) {
+#pragma unroll 16
+          for (int v = 0; v < C; ++v) walk(v);
+        } else {
+#pragma unroll 4
+          for (int v = 0; v < here; ++v) walk(v);
         }
       }
     }
   }
 #pragma unroll
   for (int o = 0; o < OWN; ++o) {
-    const int at = (int)threadIdx.x + o * 64 * NW;
-    const int m = 16 * (at >> 8) + ((at >> 2) & 15), n = n0 + 4 * ((at >> 6) & 3) + (at & 3);
-    if (at < WM * 256 && m < a.M && n < a.N) store_one<EPI>(a, m, n, acc[0][o], acc[NB - 1][o]);
+    const int e = (int)threadIdx.x + o * 64 * NW;
+    const int m = 16 * (e / PS) + ((e >> 2) & 15), n = n0 + 4 * ((e % PS) >> 6) + (e & 3);
+    if (e < OWNED && m < a.M && n < a.N) store_one<EPI>(a, m, n, acc[0][o], acc[NB - 1][o]);
   }
 }
 
 // ------------------------------------------------------------------------------ tiles
+
+// A copy made where it is written.  (A plain assignment of what a load brings becomes a copy at the loop's end, and the wait for the
+// load with it: nothing would be in flight across steps.)
+__device__ __forceinline__ float taken(float v) {
+  float r;
+  asm volatile("v_mov_b32 %0, %1" : "=v"(r) : "v"(v));
+  return r;
+}
 
 // A workgroup of eight waves computes BM rows times BN matrix rows (gated: BN / 2 gate and BN / 2 up rows) in steps of one
 // block of 128; both operands travel from memory straight into LDS, some steps ahead.  The waves lie WY x 8 / WY over the tile,
 // each with MI x NJ results of 16 x 16.  One load of a wave brings 8 rows of a step, 128 bytes each, into 1 KB of LDS, lane l's 16
 // bytes to 16 l; slot c' of row r (within its block of 16 rows) holds the row's chunk c' ^ (r >> 1), so that the 16 lanes that
 // read one chunk of 16 rows hit 16 different groups of banks.
-template <int EPI, int WY_, int MI_, int NJ_>
+template <int EPI, int WAVES_, int WY_, int MI_, int NJ_, int ST_>
 struct Fp8Tile {
-  static constexpr int WY = WY_, WX = 8 / WY_, MI = MI_, NJ = NJ_;
+  static constexpr int WAVES = WAVES_, WY = WY_, WX = WAVES / WY_, MI = MI_, NJ = NJ_, ST = ST_;
   static constexpr bool GLU = EPI == SWIGLU_FP8;
   static constexpr int BM = 16 * WY * MI, BN = 16 * WX * NJ, COLS = GLU ? BN / 2 : BN;
   static constexpr int A_SLOT = BM * 128, B_SLOT = BN * 128, STEP = A_SLOT + B_SLOT;
-  static constexpr int LA = BM / 64, LB = BN / 64;
-  static constexpr int ST = 160 * 1024 / STEP >= 4 ? 4 : 160 * 1024 / STEP;
+  static constexpr int LA = BM / (8 * WAVES), LB = BN / (8 * WAVES);
   static constexpr int BYTES = ST * STEP;
-  static_assert(BM % 64 == 0 && BN % 64 == 0 && ST >= 2 && 128 % (16 * (GLU ? NJ / 2 : NJ)) == 0 && (!GLU || COLS == 128), "tile shapes");
+  static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && ST >= 2 && BYTES <= 160 * 1024 && LA <= 8 && LB <= 8 && 128 % (16 * (GLU ? NJ / 2 : NJ)) == 0 && (!GLU || COLS == 128), "tile shapes");
 };
 
-template <int EPI, int WY, int MI, int NJ>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_fp8_tiles_kernel(Fp8Args a) {
-  using T = Fp8Tile<EPI, WY, MI, NJ>;
+template <int EPI, int WAVES, int WY, int MI, int NJ, int ST>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_fp8_tiles_kernel(Fp8Args a) {
+  using T = Fp8Tile<EPI, WAVES, WY, MI, NJ, ST>;
   constexpr bool GLU = T::GLU;
   constexpr int BM = T::BM, COLS = T::COLS, NH = GLU ? NJ / 2 : NJ, NB = GLU ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) unsigned char ring[];
@@ -231,11 +244,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int KB = a.K / BW_FP8_BLOCK;
 
   const int a_rows = min(BM, a.M - m0), b_rows = min(COLS, a.N - n0);
-  const bool up = GLU && wave >= 4;
-  const __amdgpu_buffer_rsrc_t rs_a = rows_of(a.x + (size_t)m0 * a.ldx, (size_t)(a_rows - 1) * a.ldx + a.K);
-  const __amdgpu_buffer_rsrc_t rs_b = rows_of(a.w + ((size_t)(up ? a.N : 0) + n0) * a.K, (size_t)b_rows * a.K);
+  const bool up = GLU && wave >= WAVES / 2;
+  const uint8_t* const base_a = a.x + (size_t)m0 * a.ldx;
+  const uint8_t* const base_b = a.w + ((size_t)(up ? a.N : 0) + n0) * a.K;
+  const int size_a = (a_rows - 1) * a.ldx + a.K, size_b = b_rows * a.K;
   const int lrow = lane >> 3, lslot = lane & 7;
-  int voff_a[4], voff_b[4];
+  int voff_a[8], voff_b[8];
 #pragma unroll
   for (int t = 0; t < T::LA; ++t) {
     const int row = 8 * (T::LA * wave + t) + lrow;
@@ -247,35 +261,31 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     voff_b[t] = (up ? row - COLS : row) * a.K + 16 * (lslot ^ ((row & 15) >> 1));
   }
   typedef __attribute__((address_space(3))) void* lds_ptr;
+  // (a step past the end: descriptors without a byte, no traffic, zeros into a slot that nobody reads)
   auto issue = [&](int step, int slot) {
+    const bool live = step < KB;
+    const __amdgpu_buffer_rsrc_t rs_a = rows_of(base_a, live ? size_a : 0), rs_b = rows_of(base_b, live ? size_b : 0);
+    unsigned char* const to = ring + slot * T::STEP;
 #pragma unroll
     for (int t = 0; t < T::LA; ++t)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_a, (lds_ptr)(ring + slot * T::STEP + (T::LA * wave + t) * 1024), 16,
-                                               step < KB ? voff_a[t] : OUTSIDE, step * 128, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_a, (lds_ptr)(to + (T::LA * wave + t) * 1024), 16, voff_a[t], step * 128, 0, 0);
 #pragma unroll
     for (int t = 0; t < T::LB; ++t)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_b, (lds_ptr)(ring + slot * T::STEP + T::A_SLOT + (T::LB * wave + t) * 1024), 16,
-                                               step < KB ? voff_b[t] : OUTSIDE, step * 128, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_b, (lds_ptr)(to + T::A_SLOT + (T::LB * wave + t) * 1024), 16, voff_b[t], step * 128, 0, 0);
   };
-  // the scales of this wave's rows and columns for a step
-  int row_m[8];
+  // The scales of this wave's rows and columns for a step, asked for a step ahead (rows past M: zeros).
+  const int xs_at = 4 * (m0 + 16 * MI * wy + r);
+  const int NBLK = (a.N + BW_FP8_BLOCK - 1) / BW_FP8_BLOCK;
+  const int my_block = min((n0 + 16 * NH * wx) / BW_FP8_BLOCK, NBLK - 1);       // (columns past the matrix: any scale will do)
+  const float* xs_step = a.xs;
+  const float* ws_step = a.ws + (size_t)my_block * KB;
+  float sx[8], sw[2], sx_next[8], sw_next[2];
+  auto scales = [&]() {
+    const __amdgpu_buffer_rsrc_t rs = rows_of(xs_step, (size_t)a.M * 4);
 #pragma unroll
-  for (int i = 0; i < MI; ++i) row_m[i] = min(m0 + 16 * (MI * wy + i) + r, a.M - 1);
-  const float* ws_row[NB];
+    for (int i = 0; i < MI; ++i) sx_next[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, xs_at + 64 * i, 0, 0));
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
-    ws_row[b] = a.ws + ((size_t)((n0 + 16 * NH * wx) / BW_FP8_BLOCK) + (size_t)b * ((a.N + BW_FP8_BLOCK - 1) / BW_FP8_BLOCK)) * KB;
-  if (n0 + 16 * NH * wx >= a.N) {               // (columns past the matrix: any scale will do)
-#pragma unroll
-    for (int b = 0; b < NB; ++b) ws_row[b] = a.ws;
-  }
-  float sx[8], sw[2];
-  auto scales = [&](int step) {
-    const int s = min(step, KB - 1);
-#pragma unroll
-    for (int i = 0; i < MI; ++i) sx[i] = a.xs[(size_t)s * a.ldxs + row_m[i]];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) sw[b] = ws_row[b][s];
+    for (int b = 0; b < NB; ++b) sw_next[b] = ws_step[(size_t)b * NBLK * KB];
   };
 
   f32x4 acc[MI][NJ];
@@ -287,51 +297,155 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   int slot_off[2];
 #pragma unroll
   for (int kk = 0; kk < 2; ++kk) slot_off[kk] = row_off + (((4 * kk + g) ^ (r >> 1)) * 16);
-
-  scales(0);
-#pragma unroll
-  for (int st = 0; st < T::ST - 1; ++st) issue(st, st);
-  int slot = 0;
-  for (int step = 0; step < KB; ++step) {
-    // all but the loads of the ST - 2 steps behind this one
-    __builtin_amdgcn_s_waitcnt(vmcnt_only((T::ST - 2) * (T::LA + T::LB)) & ~0x0f00);
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    float f[8][2];
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int b = 0; b < NB; ++b) f[i][b] = sx[i] * sw[b];
-    scales(step + 1);
-    issue(step + T::ST - 1, slot == 0 ? T::ST - 1 : slot - 1);
-    const unsigned char* at_a = ring + slot * T::STEP;
-    const unsigned char* at_b = at_a + T::A_SLOT;
-    Frag fb[NJ];
+  // Operands as they come from LDS (of a block of x, of a half of the wave's blocks of the matrix), converted, and the results of
+  // the block of x at hand and of the one before.
+  u32x4 ra[2], rb[NJ];
+  Frag fa, fb[NJ];
+  constexpr int PN = MI > 4 ? 1 : 2;
+  f32x4 p[2][NJ];
+  auto read_a = [&](int at_slot, int i, int kk) {
+    ra[kk] = *reinterpret_cast<const u32x4*>(ring + at_slot * T::STEP + (MI * wy + i) * 2048 + slot_off[kk]);
+  };
+  auto read_b = [&](int at_slot, int kk) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int blk = GLU ? (NH * wx + j % NH) + (j / NH) * (T::BN / 32) : NJ * wx + j;
-      fb[j] = frag_of(*reinterpret_cast<const u32x4*>(at_b + blk * 2048 + slot_off[0]), *reinterpret_cast<const u32x4*>(at_b + blk * 2048 + slot_off[1]));
+      rb[j] = *reinterpret_cast<const u32x4*>(ring + at_slot * T::STEP + T::A_SLOT + blk * 2048 + slot_off[kk]);
     }
+  };
+  auto add_up = [&](int i, int e) {                               // element e of block i's results joins its chain
+    const int j = e >> 2, q = e & 3;
+    acc[i][j][q] = fmaf(sx[i] * sw[GLU ? j / NH : 0], p[PN == 1 ? 0 : i & 1][j][q], acc[i][j][q]);
+  };
+
+  scales();
+#pragma unroll
+  for (int st = 0; st < T::ST; ++st) issue(st, st);
+  __builtin_amdgcn_s_waitcnt(vmcnt_only((T::ST - 1) * (T::LA + T::LB)));
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  read_b(0, 0);
+  read_a(0, 0, 0);
+  read_a(0, 0, 1);
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) fb[j].t[t] = quarter_of(rb[j], t);
+#pragma unroll
+  for (int t = 0; t < 3; ++t) fa.t[t] = quarter_of(ra[t >> 1], t & 1);
+  read_b(0, 1);
+  read_a(0, 1, 0);
+#pragma unroll
+  for (int i = 0; i < MI; ++i) sx[i] = 0.0f;                       // (the first block adds up a block that was none)
+  sw[0] = sw[1] = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) p[PN - 1][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  int slot = 0;
+  for (int step = 0; step < KB; ++step) {
+    const int next = slot + 1 == T::ST ? 0 : slot + 1;
+    // A step is MI blocks of x, a block four phases: a quarter of the block's k against the wave's NJ blocks of the matrix.  Under a
+    // phase's matrix instructions a quarter of the block before joins the chains and what the phase before was the last to use is
+    // replaced by what comes next (a quarter of the next block of x; in the step's last phases and the next one's first, of the
+    // matrix's blocks).  The barrier stands a block and a half before the step's end, when the wave has its last operands of the step.
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-      const unsigned char* at = at_a + (MI * wy + i) * 2048;
-      const Frag fa = frag_of(*reinterpret_cast<const u32x4*>(at + slot_off[0]), *reinterpret_cast<const u32x4*>(at + slot_off[1]));
-      f32x4 p[NJ];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) p[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < 4; ++t) {
+        int valu = 0, reads = 0;
+        __builtin_amdgcn_sched_barrier(0);
+        if (i == MI - 2 && t == 2) {
+          __builtin_amdgcn_s_waitcnt(vmcnt_only((T::ST - 2) * (T::LA + T::LB)) & ~0x0f00);
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+          issue(step + T::ST, slot);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        // reads: the next block of x, its second half two phases behind its first; the next step's halves of the matrix's blocks
+        const int from = i + 1 < MI ? slot : next;
+        if (t == 1) {
+          read_a(from, (i + 1) % MI, 1);
+          reads += 1;
+        }
+        if (t == 3) {
+          read_a(i + 2 < MI ? slot : next, (i + 2) % MI, 0);
+          reads += 1;
+          if (i == MI - 2) {
+            read_b(next, 0);
+            reads += NJ;
+          }
+        }
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+        for (int j = 0; j < NJ; ++j) {
+          constexpr int at = 0;
+          f32x4& pj = p[PN == 1 ? at : i & 1][j];
+          if (PN == 1 && t == 0) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) p[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j].t[t], fa.t[t], p[j], 0, 0, 0);
+            for (int q = 0; q < 4; ++q) add_up((i + MI - 1) % MI, 4 * j + q);
+          }
+          if (t == 0) pj = (f32x4){0.f, 0.f, 0.f, 0.f};
+          pj = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j].t[t], fa.t[t], pj, 0, 0, 0);
+        }
+        if (PN == 2) {
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const float s = f[i][GLU ? j / NH : 0];
+          for (int e = t * NJ; e < (t + 1) * NJ; ++e) add_up((i + MI - 1) % MI, e);
+          valu += NJ;
+        } else if (t == 0) {
+          valu += 4 * NJ;
+        }
+        // (the quarter that this phase's instructions are the last to use is replaced a phase later)
+        const int was = (t + 3) & 3;
+        fa.t[was] = quarter_of(ra[was >> 1], was & 1);
+        valu += 4;
+        if (i == MI - 1 && t == 1) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[i][j][q] = fmaf(s, p[j][q], acc[i][j][q]);
+          for (int j = 0; j < NJ; ++j) fb[j].t[0] = quarter_of(rb[j], 0);
+          valu += 4 * NJ;
+        }
+        if (i == MI - 1 && t == 2) {
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) fb[j].t[1] = quarter_of(rb[j], 1);
+          valu += 4 * NJ;
+        }
+        if (i == MI - 1 && t == 3) {
+          read_b(next, 1);
+          reads += NJ;
+        }
+        if (i == 0 && t == 0) {
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) fb[j].t[2] = quarter_of(rb[j], 0);
+          valu += 4 * NJ;
+        }
+        if (i == 0 && t == 1) {
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) fb[j].t[3] = quarter_of(rb[j], 1);
+          valu += 4 * NJ;
+        }
+#pragma unroll
+        for (int k = 0; k < NJ; ++k) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          if (k == 0 && reads) __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+          if (valu > 4 * NJ) __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+          else __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+        }
+        if (i == 0 && t == 3) {
+          // every result of the step before has joined its chain
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int k = 0; k < MI; ++k) sx[k] = taken(sx_next[k]);
+#pragma unroll
+          for (int b = 0; b < NB; ++b) sw[b] = taken(sw_next[b]);
+          if (step + 1 < KB) {
+            xs_step += a.ldxs;
+            ws_step += 1;
+          }
+          scales();
+        }
       }
     }
-    slot = slot + 1 == T::ST ? 0 : slot + 1;
+    slot = next;
   }
+#pragma unroll
+  for (int e = 0; e < 4 * NJ; ++e) add_up(MI - 1, e);
   __builtin_amdgcn_s_waitcnt(vmcnt_only(0));                       // the padding loads too, before LDS is used again or the waves end
 
   if constexpr (GLU) {
@@ -356,6 +470,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       if (g == 0) most[wx * BM + 16 * (MI * wy + i) + r] = mx;
     }
     __syncthreads();
+// The codes of the tile's rows lie in LDS row by row (144 bytes apart, which spreads the columns' words over the banks) and
+    // leave as whole lines.
+    constexpr int CODES_AT = 4 * T::WX * BM, CLD = 144;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const int row = 16 * (MI * wy + i) + r, m = m0 + row;
@@ -364,57 +481,172 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       for (int v = 0; v < T::WX; ++v) mx = max_bits(mx, most[v * BM + row]);
       const float scale = fp8_scale_of(mx);
       const float inv = 1.0f / scale;
-      if (m < a.M) {
 #pragma unroll
-        for (int j = 0; j < NH; ++j)
-          *reinterpret_cast<uint32_t*>((uint8_t*)a.out + (size_t)m * a.ldo + n0 + 16 * (NH * wx + j) + 4 * g) =
-              fp8_codes4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], inv);
-        if (wx == 0 && g == 0) a.out_scales[(size_t)(n0 / BW_FP8_BLOCK) * a.lds + m] = scale;
-      }
+      for (int j = 0; j < NH; ++j)
+        *reinterpret_cast<uint32_t*>(ring + CODES_AT + row * CLD + 16 * (NH * wx + j) + 4 * g) =
+            fp8_codes4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], inv);
+      if (m < a.M && wx == 0 && g == 0) a.out_scales[(size_t)(n0 / BW_FP8_BLOCK) * a.lds + m] = scale;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < BM * 8 / (64 * WAVES); ++e) {
+      const int at = e * 64 * WAVES + (int)threadIdx.x, row = at >> 3, m = m0 + row;
+      if (m < a.M)
+        *reinterpret_cast<u32x4*>((uint8_t*)a.out + (size_t)m * a.ldo + n0 + 16 * (at & 7)) =
+            *reinterpret_cast<const u32x4*>(ring + CODES_AT + row * CLD + 16 * (at & 7));
     }
   } else {
+    // 16 rows of the wave's results at a time go through LDS of its own, so that a store covers whole rows of them: a lane holds
+    // four neighbours of one of 16 rows.
+    __syncthreads();
+    constexpr int W = 16 * NJ, LDW = W + 4;
+    float* const mine = reinterpret_cast<float*>(ring) + wave * 16 * LDW;
+    const int nw = n0 + W * wx;
+    constexpr int PER = EPI == STORE_BF16 ? 8 : 4, LANES = W / PER, ROWS = 64 / LANES;      // elements a lane, lanes a row, rows a store
+    const bool vec = a.vec_out && nw + W <= a.N;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-      const int m = m0 + 16 * (MI * wy + i) + r;
-      if (m >= a.M) continue;
+      const int m1 = m0 + 16 * (MI * wy + i);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
+      for (int j = 0; j < NJ; ++j) *reinterpret_cast<f32x4*>(mine + r * LDW + 16 * j + 4 * g) = acc[i][j];
+      __builtin_amdgcn_wave_barrier();
+      if (vec) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = n0 + 16 * (NJ * wx + j) + 4 * g + q;
-          if (n < a.N) store_one<EPI>(a, m, n, acc[i][j][q], 0.0f);
+        for (int e = 0; e < 16 / ROWS; ++e) {
+          const int row = e * ROWS + lane / LANES, c = PER * (lane % LANES), m = m1 + row;
+          f32x4 y = *reinterpret_cast<const f32x4*>(mine + row * LDW + c);
+          if constexpr (EPI == STORE_BF16) {
+            const f32x4 z = *reinterpret_cast<const f32x4*>(mine + row * LDW + c + 4);
+            if (m < a.M)
+              *reinterpret_cast<u32x4*>((bf16_t*)a.out + (size_t)m * a.ldo + nw + c) =
+                  (u32x4){pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3])};
+          } else if (m < a.M) {
+            if (a.residual != nullptr) y = *reinterpret_cast<const f32x4*>(a.residual + (size_t)m * a.ldr + nw + c) + y;
+            *reinterpret_cast<f32x4*>((float*)a.out + (size_t)m * a.ldo + nw + c) = y;
+          }
         }
+      } else {
+        constexpr int RPS = 64 / W;                                  // rows a store of single elements
+#pragma unroll 4
+        for (int e = 0; e < 16 / RPS; ++e) {
+          const int row = e * RPS + lane / W, c = lane % W;
+          if (m1 + row < a.M && nw + c < a.N) store_one<EPI>(a, m1 + row, nw + c, mine[row * LDW + c], 0.0f);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
     }
   }
 }
 
 // ------------------------------------------------------------------------------ which kernel
 
+template <int WM, int EPI, int NW, int D, int CW>
+int launch_few(const Fp8Args& a, hipStream_t s) {
+  constexpr int NB = EPI == SWIGLU_F32 ? 2 : 1, LDS = NW * D * NB * WM * 16 * (CW + 1) * 4;
+  static_assert(LDS <= 160 * 1024, "a pass's sums fit LDS");
+  hipLaunchKernelGGL((gemm_fp8_few_kernel<WM, EPI, NW, D, CW>), dim3((a.N + CW - 1) / CW), dim3(64 * NW), LDS, s, a);
+  return BW_LAUNCH_CHECK();
+}
+
+// Strips of 16 columns for the 256 compute units, K's blocks over the waves of one.  Eight waves a strip where there are strips for
+// more than one workgroup a unit (8 rows of 28672 columns, K = 4096: 27.0 us, with 16 waves 28.2), 16 where there is about one
+// (4096 columns, K = 8192: 10.4, with eight 10.8; 64 rows, K = 4096: 12.9 and 13.3).  Up to 2048 columns of at most 16 rows strips of
+// eight, so that every unit has one: of 2048 columns, K = 2048, 3.4 us for 3.7, K = 8192 with all of K asked for at once by 16 waves 8.3
+// for 9.8, with eight waves 9.0 (K = 2048 so 5.8: most waves have nothing).
 template <int WM, int EPI>
-void launch_few(const Fp8Args& a, hipStream_t s) {
-  constexpr int NW = EPI == SWIGLU_F32 ? (WM == 1 ? 8 : 4) : (WM <= 2 ? 8 : 4);
-  constexpr int D = WM == 1 ? 4 : 2;
-  hipLaunchKernelGGL((gemm_fp8_few_kernel<WM, EPI, NW, D>), dim3((a.N + 15) / 16), dim3(64 * NW), 0, s, a);
+int few_rows_as(const Fp8Args& a, hipStream_t s) {
+  const int KB = a.K / BW_FP8_BLOCK;
+  if constexpr (WM == 1) {
+    if (a.N <= 2048) {
+      if constexpr (EPI != SWIGLU_F32) {
+        if (KB > 32 && KB <= 64) return launch_few<WM, EPI, 16, 4, 8>(a, s);
+      }
+      return launch_few<WM, EPI, 8, 2, 8>(a, s);
+    }
+  }
+  if constexpr (EPI != SWIGLU_F32) {
+    if (a.N <= 5120) return launch_few<WM, EPI, 16, 1, 16>(a, s);
+  }
+  return launch_few<WM, EPI, 8, 1, 16>(a, s);
 }
 
 template <int EPI>
 int few_rows(const Fp8Args& a, hipStream_t s) {
   switch ((a.M + 15) / 16) {
-    case 1: launch_few<1, EPI>(a, s); break;
-    case 2: launch_few<2, EPI>(a, s); break;
-    case 3: launch_few<3, EPI>(a, s); break;
-    default: launch_few<4, EPI>(a, s); break;
+    case 1: return few_rows_as<1, EPI>(a, s);
+    case 2: return few_rows_as<2, EPI>(a, s);
+    case 3: return few_rows_as<3, EPI>(a, s);
+    default: return few_rows_as<4, EPI>(a, s);
   }
+}
+
+template <int EPI, int WAVES, int WY, int MI, int NJ, int ST>
+int launch_tiles(Fp8Args a, hipStream_t s) {
+  using T = Fp8Tile<EPI, WAVES, WY, MI, NJ, ST>;
+  a.m_tiles = (a.M + T::BM - 1) / T::BM;
+  a.n_tiles = (a.N + T::COLS - 1) / T::COLS;
+  hipLaunchKernelGGL((gemm_fp8_tiles_kernel<EPI, WAVES, WY, MI, NJ, ST>), dim3((unsigned)(a.m_tiles * a.n_tiles)), dim3(64 * T::WAVES), T::BYTES, s, a);
   return BW_LAUNCH_CHECK();
 }
 
-template <int EPI, int WY, int MI, int NJ>
-int launch_tiles(Fp8Args a, hipStream_t s) {
-  using T = Fp8Tile<EPI, WY, MI, NJ>;
-  a.m_tiles = (a.M + T::BM - 1) / T::BM;
-  a.n_tiles = (a.N + T::COLS - 1) / T::COLS;
-  hipLaunchKernelGGL((gemm_fp8_tiles_kernel<EPI, WY, MI, NJ>), dim3((unsigned)(a.m_tiles * a.n_tiles)), dim3(512), T::BYTES, s, a);
-  return BW_LAUNCH_CHECK();
+// What a shape of tile takes, in us: a workgroup's start and end, and a step of 128 of K, with the compute unit for itself and, where
+// two fit (``per_cu`` 2), beside another.  Measured on normal values (the power of the matrix cores, and with it their clock, hangs
+// on them): slopes over K = 2048 and 8192, grids of up to 256 workgroups and of one or two full rounds.
+struct TileCost {
+  int rows, columns, per_cu;
+  double start, step, start_beside, step_beside;
+};
+
+double tiles_us(const TileCost& c, int M, int N, int K) {
+  const double steps = K / BW_FP8_BLOCK, alone = c.start + steps * c.step, beside = c.start_beside + steps * c.step_beside;
+  const long long tiles = (long long)((M + c.rows - 1) / c.rows) * ((N + c.columns - 1) / c.columns);
+  const long long full = tiles / (256 * c.per_cu), rest = tiles % (256 * c.per_cu);
+  return 2.5 + full * (c.per_cu == 2 ? beside : alone) + (rest == 0 ? 0.0 : rest <= 256 ? alone : beside);
+}
+
+// Few rows: the matrix from memory (4.2 MB a us, the first byte included) and every strip's x from the L2s (7.2 MB a us), by as many units as there
+// are strips.
+double few_us(int M, int N, int K, int halves) {
+  const double strips = (N + 15) / 16, mb = 1e-6 * K * N;
+  return 1.5 + (mb * halves / 4.2 + 1e-6 * strips * M * K / 7.2) * (strips < 256 ? 256 / strips : 1.0);
+}
+
+template <int SHAPES>
+int cheapest(const TileCost (&shapes)[SHAPES], int M, int N, int K, double* us) {
+  int best = 0;
+  *us = tiles_us(shapes[0], M, N, K);
+  for (int i = 1; i < SHAPES; ++i) {
+    const double t = tiles_us(shapes[i], M, N, K);
+    if (t < *us) {
+      *us = t;
+      best = i;
+    }
+  }
+  return best;
+}
+
+// A step's conversions a matrix instruction fall with the tile: 192 x 256 a workgroup of eight waves does the most a us, 128 x 128 by
+// four waves, two workgroups a unit, fills a round sooner, 64 x 128 and 64 x 64 give a few hundred rows of few columns more workgroups.
+constexpr TileCost STORE_SHAPES[] = {{192, 256, 1, 6.0, 2.04, 0, 0}, {128, 128, 2, 5.3, 1.02, 6.0, 1.78}, {64, 128, 2, 2.4, 0.64, 2.6, 1.12}, {64, 64, 2, 2.0, 0.49, 2.7, 0.74}};
+constexpr TileCost GATED_SHAPES[] = {{192, 128, 1, 10.5, 2.04, 0, 0}, {128, 128, 1, 5.0, 1.70, 0, 0}, {64, 128, 2, 3.0, 1.20, 9.0, 1.60}, {32, 128, 2, 2.0, 0.95, 4.0, 1.30}};
+
+template <int EPI>
+int stored_by_tiles(const Fp8Args& a, int shape, hipStream_t s) {
+  switch (shape) {
+    case 0: return launch_tiles<EPI, 8, 2, 6, 4, 2>(a, s);
+    case 1: return launch_tiles<EPI, 4, 2, 4, 4, 2>(a, s);
+    case 2: return launch_tiles<EPI, 4, 2, 2, 4, 3>(a, s);
+    default: return launch_tiles<EPI, 4, 2, 2, 2, 4>(a, s);
+  }
+}
+
+int gated_by_tiles(const Fp8Args& a, int shape, hipStream_t s) {
+  switch (shape) {
+    case 0: return launch_tiles<SWIGLU_FP8, 8, 2, 6, 4, 2>(a, s);
+    case 1: return launch_tiles<SWIGLU_FP8, 8, 2, 4, 4, 3>(a, s);
+    case 2: return launch_tiles<SWIGLU_FP8, 4, 1, 4, 4, 2>(a, s);
+    default: return launch_tiles<SWIGLU_FP8, 4, 1, 2, 4, 2>(a, s);
+  }
 }
 
 bool aligned(const void* p, int n) { return ((uintptr_t)p & (n - 1)) == 0; }
@@ -440,10 +672,13 @@ extern "C" int bw_gemm_fp8(const void* x, int ldx, const float* xs, int ldxs, co
   Fp8Args a = {};
   a.x = (const uint8_t*)x, a.xs = xs, a.w = (const uint8_t*)w, a.ws = ws, a.residual = residual, a.out = out;
   a.ldx = ldx, a.ldxs = ldxs, a.ldr = ldr, a.ldo = ldo, a.M = rows, a.N = N, a.K = K;
+  a.vec_out = aligned(out, 16) && (rows == 1 || (long long)ldo * (out_is_bf16 ? 2 : 4) % 16 == 0) &&
+              (residual == nullptr || (aligned(residual, 16) && (rows == 1 || ldr % 4 == 0)));
   hipStream_t s = (hipStream_t)stream;
-  if (rows <= FEW_ROWS) return out_is_bf16 ? few_rows<STORE_BF16>(a, s) : few_rows<STORE_F32>(a, s);
-  if (out_is_bf16) return launch_tiles<STORE_BF16, 2, 4, 4>(a, s);
-  return launch_tiles<STORE_F32, 2, 4, 4>(a, s);
+  double us;
+  const int shape = cheapest(STORE_SHAPES, rows, N, K, &us);
+  if (rows <= 16 || (rows <= FEW_ROWS && few_us(rows, N, K, 1) <= us)) return out_is_bf16 ? few_rows<STORE_BF16>(a, s) : few_rows<STORE_F32>(a, s);
+  return out_is_bf16 ? stored_by_tiles<STORE_BF16>(a, shape, s) : stored_by_tiles<STORE_F32>(a, shape, s);
 }
 
 extern "C" int bw_gemm_fp8_swiglu(const void* x, int ldx, const float* xs, int ldxs, const void* w, const float* ws, float* sums, int ldsums, void* codes,
@@ -457,12 +692,16 @@ extern "C" int bw_gemm_fp8_swiglu(const void* x, int ldx, const float* xs, int l
   a.x = (const uint8_t*)x, a.xs = xs, a.w = (const uint8_t*)w, a.ws = ws;
   a.ldx = ldx, a.ldxs = ldxs, a.M = rows, a.N = inter, a.K = K;
   hipStream_t s = (hipStream_t)stream;
+  double us;
+  const int shape = cheapest(GATED_SHAPES, rows, inter, K, &us);
   if (rows <= FEW_ROWS) {
     if (sums == nullptr || (rows > 1 && ldsums < inter)) return -2;
-    a.out = sums, a.ldo = ldsums;
-    if (const int bad = few_rows<SWIGLU_F32>(a, s)) return bad;
-    return bw_quantize_fp8(sums, 0, ldsums, codes, ldq, scales, lds, rows, inter, stream);
+    if (rows <= 16 || few_us(rows, inter, K, 2) + 2.5 <= us) {         // (the quantization of the sums is a launch of its own)
+      a.out = sums, a.ldo = ldsums;
+      if (const int bad = few_rows<SWIGLU_F32>(a, s)) return bad;
+      return bw_quantize_fp8(sums, 0, ldsums, codes, ldq, scales, lds, rows, inter, stream);
+    }
   }
   a.out = codes, a.ldo = ldq, a.out_scales = scales, a.lds = lds;
-  return launch_tiles<SWIGLU_FP8, 2, 4, 4>(a, s);
+  return gated_by_tiles(a, shape, s);
 }
