@@ -95,43 +95,46 @@ __device__ __forceinline__ void store_one(const Fp8Args& a, int m, int n, float 
 
 // ------------------------------------------------------------------------------ few rows
 
-// Up to 64 rows: a workgroup of NW waves a strip of CW matrix rows (gated: CW gate and CW up rows).  The blocks of K go round the
-// waves, D to a wave and pass, all asked for before any is waited for; their sums meet in LDS, where the threads that own the outputs
-// walk them in order.  CW = 8 halves the strip (lanes with r >= 8 ask for nothing): twice as many workgroups, for products with too
-// few columns to give every compute unit 16.
-template <int WM, int EPI, int NW, int D, int CW>
+// A workgroup of NW waves a block of 16 WM rows of x and NC strips of CW matrix rows (gated: as many gate and up rows).  The blocks of
+// K go round the waves, D to a wave and pass, all asked for before any is waited for; their sums meet in LDS, where the threads that
+// own the outputs walk them in order.  CW = 8 halves a strip (lanes with r >= 8 ask for nothing): twice as many workgroups, for
+// products with too few columns to give every compute unit 16.  More strips a workgroup share x's loads and its conversion.
+template <int WM, int NC, int EPI, int NW, int D, int CW>
 __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
-  constexpr int NB = EPI == SWIGLU_F32 ? 2 : 1;
-  constexpr int PS = 16 * CW, OWNED = WM * PS, OWN = (OWNED + 64 * NW - 1) / (64 * NW), C = NW * D;
-  extern __shared__ __attribute__((aligned(16))) float part[];                  // [C][NB][WM][PS], then the factors
-  float* factor = part + C * NB * WM * PS;                                      // [C][NB][WM * 16]
+  constexpr int NB = EPI == SWIGLU_F32 ? 2 : 1, NS = NB * NC;                    // (strip c of gate or up b: c * NB + b)
+  constexpr int PS = 16 * CW, OWNED = NC * WM * PS, OWN = (OWNED + 64 * NW - 1) / (64 * NW), C = NW * D;
+  extern __shared__ __attribute__((aligned(16))) float part[];                  // [C][NB][NC][WM][PS], then the factors
+  float* factor = part + C * NB * OWNED;                                        // [C][NB][WM * 16]
   const int wave = wave_index(), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * CW, KB = a.K / BW_FP8_BLOCK;
-  const int w_rows = min(CW, a.N - n0);
+  const int n0 = blockIdx.x * (CW * NC), m0 = blockIdx.y * (16 * WM), KB = a.K / BW_FP8_BLOCK;
+  const int rows = min(16 * WM, a.M - m0);
   __amdgpu_buffer_rsrc_t rs_w[NB];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) rs_w[b] = rows_of(a.w + ((size_t)b * a.N + n0) * a.K, (size_t)w_rows * a.K);
-  const __amdgpu_buffer_rsrc_t rs_x = rows_of(a.x, (size_t)(a.M - 1) * a.ldx + a.K);
+  for (int b = 0; b < NB; ++b) rs_w[b] = rows_of(a.w + ((size_t)b * a.N + n0) * a.K, (size_t)min(CW * NC, a.N - n0) * a.K);
+  const __amdgpu_buffer_rsrc_t rs_x = rows_of(a.x + (size_t)m0 * a.ldx, (size_t)(rows - 1) * a.ldx + a.K);
   const int voff_w = r < CW ? r * a.K + 16 * g : OUTSIDE;
   int voff_x[WM], row_m[WM];
 #pragma unroll
   for (int i = 0; i < WM; ++i) {
-    voff_x[i] = 16 * i + r < a.M ? (16 * i + r) * a.ldx + 16 * g : OUTSIDE;
-    row_m[i] = min(16 * i + r, a.M - 1);
+    voff_x[i] = 16 * i + r < rows ? (16 * i + r) * a.ldx + 16 * g : OUTSIDE;
+    row_m[i] = m0 + min(16 * i + r, rows - 1);
   }
   const float* ws_row[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) ws_row[b] = a.ws + ((size_t)(n0 / BW_FP8_BLOCK) + (size_t)b * ((a.N + BW_FP8_BLOCK - 1) / BW_FP8_BLOCK)) * KB;
 
-  u32x4 wq[D][NB][2], xq[D][WM][2];
+  u32x4 wq[D][NS][2], xq[D][WM][2];
   float sx[D][WM], sw[D][NB];
   auto issue = [&](int d, int pass) {
     const int blk = min((pass * D + d) * NW + wave, KB - 1);     // (past the end: the last block again, whose sums nobody takes)
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      wq[d][b][0] = __builtin_amdgcn_raw_buffer_load_b128(rs_w[b], voff_w, blk * BW_FP8_BLOCK, 0);
-      wq[d][b][1] = __builtin_amdgcn_raw_buffer_load_b128(rs_w[b], voff_w + 64, blk * BW_FP8_BLOCK, 0);
-    }
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int at = voff_w + c * CW * a.K;                    // (a strip past the matrix lies outside the descriptor)
+        wq[d][c * NB + b][0] = __builtin_amdgcn_raw_buffer_load_b128(rs_w[b], at, blk * BW_FP8_BLOCK, 0);
+        wq[d][c * NB + b][1] = __builtin_amdgcn_raw_buffer_load_b128(rs_w[b], at + 64, blk * BW_FP8_BLOCK, 0);
+      }
 #pragma unroll
     for (int i = 0; i < WM; ++i) {
       xq[d][i][0] = __builtin_amdgcn_raw_buffer_load_b128(rs_x, voff_x[i], blk * BW_FP8_BLOCK, 0);
@@ -157,16 +160,19 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
     for (int d = 0; d < D; ++d) {
       const int at = d * NW + wave;
       if (pass * C + at < KB) {                                  // (scalar)
-        Frag fw[NB];
+        Frag fw[NS];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) fw[b] = frag_of(wq[d][b][0], wq[d][b][1]);
+        for (int k = 0; k < NS; ++k) fw[k] = frag_of(wq[d][k][0], wq[d][k][1]);
 #pragma unroll
         for (int i = 0; i < WM; ++i) {
           const Frag fx = frag_of(xq[d][i][0], xq[d][i][1]);
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
-            const f32x4 sums = block_sums(fw[b], fx);
-            if (CW == 16 || lane < 32) *reinterpret_cast<f32x4*>(part + ((at * NB + b) * WM + i) * PS + 4 * lane) = sums;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              const f32x4 sums = block_sums(fw[c * NB + b], fx);
+              if (CW == 16 || lane < 32) *reinterpret_cast<f32x4*>(part + (((at * NB + b) * NC + c) * WM + i) * PS + 4 * lane) = sums;
+            }
             if (g == 0) factor[(at * NB + b) * (WM * 16) + 16 * i + r] = sx[d][i] * sw[d][b];
           }
         }
@@ -180,10 +186,10 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
     for (int o = 0; o < OWN; ++o) {
       const int e = (int)threadIdx.x + o * 64 * NW;
       if (e < OWNED) {
-        const int m = 16 * (e / PS) + ((e >> 2) & 15);
+        const int m = 16 * (e / PS % WM) + ((e >> 2) & 15);
         auto walk = [&](int v) {
 #pragma unroll
-          for (int b = 0; b < NB; ++b) acc[b][o] = fmaf(factor[(v * NB + b) * (WM * 16) + m], part[(v * NB + b) * (WM * PS) + e], acc[b][o]);
+          for (int b = 0; b < NB; ++b) acc[b][o] = fmaf(factor[(v * NB + b) * (WM * 16) + m], part[(v * NB + b) * OWNED + e], acc[b][o]);
         };
         if (here == C) {
 #pragma unroll 16
@@ -198,7 +204,7 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
 #pragma unroll
   for (int o = 0; o < OWN; ++o) {
     const int e = (int)threadIdx.x + o * 64 * NW;
-    const int m = 16 * (e / PS) + ((e >> 2) & 15), n = n0 + 4 * ((e % PS) >> 6) + (e & 3);
+    const int m = m0 + 16 * (e / PS % WM) + ((e >> 2) & 15), n = n0 + CW * (e / (PS * WM)) + 4 * ((e % PS) >> 6) + (e & 3);
     if (e < OWNED && m < a.M && n < a.N) store_one<EPI>(a, m, n, acc[0][o], acc[NB - 1][o]);
   }
 }
@@ -540,43 +546,44 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 
 // ------------------------------------------------------------------------------ which kernel
 
-template <int WM, int EPI, int NW, int D, int CW>
+template <int WM, int NC, int EPI, int NW, int D, int CW>
 int launch_few(const Fp8Args& a, hipStream_t s) {
-  constexpr int NB = EPI == SWIGLU_F32 ? 2 : 1, LDS = NW * D * NB * WM * 16 * (CW + 1) * 4;
-  static_assert(LDS <= 160 * 1024, "a pass's sums fit LDS");
-  hipLaunchKernelGGL((gemm_fp8_few_kernel<WM, EPI, NW, D, CW>), dim3((a.N + CW - 1) / CW), dim3(64 * NW), LDS, s, a);
+  constexpr int NB = EPI == SWIGLU_F32 ? 2 : 1, LDS = NW * D * NB * WM * 16 * (CW * NC + 1) * 4;
+  static_assert(LDS <= 160 * 1024 && 128 % (CW * NC) == 0, "a pass's sums fit LDS, a workgroup's columns one block's scale");
+  hipLaunchKernelGGL((gemm_fp8_few_kernel<WM, NC, EPI, NW, D, CW>), dim3((a.N + CW * NC - 1) / (CW * NC), (a.M + 16 * WM - 1) / (16 * WM)), dim3(64 * NW), LDS, s,
+                     a);
   return BW_LAUNCH_CHECK();
 }
 
-// Strips of 16 columns for the 256 compute units, K's blocks over the waves of one.  Eight waves a strip where there are strips for
-// more than one workgroup a unit (8 rows of 28672 columns, K = 4096: 27.0 us, with 16 waves 28.2), 16 where there is about one
-// (4096 columns, K = 8192: 10.4, with eight 10.8; 64 rows, K = 4096: 12.9 and 13.3).  Up to 2048 columns of at most 16 rows strips of
-// eight, so that every unit has one: of 2048 columns, K = 2048, 3.4 us for 3.7, K = 8192 with all of K asked for at once by 16 waves 8.3
-// for 9.8, with eight waves 9.0 (K = 2048 so 5.8: most waves have nothing).
-template <int WM, int EPI>
-int few_rows_as(const Fp8Args& a, hipStream_t s) {
+// Up to 16 rows: strips of 16 columns for the 256 compute units, K's blocks over the waves of one.  Eight waves a strip where there are
+// strips for more than one workgroup a unit (8 rows of 28672 columns, K = 4096: 27.0 us, with 16 waves 28.2), 16 where there is about
+// one (4096 columns, K = 8192: 10.4, with eight 10.8).  Up to 2048 columns strips of eight, so that every unit has one: of 2048 columns,
+// K = 2048, 3.4 us for 3.7; K = 8192 with all of K asked for at once by 16 waves 8.3 for 9.8, with eight waves 9.0 (K = 2048 so 5.8:
+// most waves have nothing).
+template <int EPI>
+int sixteen_rows(const Fp8Args& a, hipStream_t s) {
   const int KB = a.K / BW_FP8_BLOCK;
-  if constexpr (WM == 1) {
-    if (a.N <= 2048) {
-      if constexpr (EPI != SWIGLU_F32) {
-        if (KB > 32 && KB <= 64) return launch_few<WM, EPI, 16, 4, 8>(a, s);
-      }
-      return launch_few<WM, EPI, 8, 2, 8>(a, s);
+  if (a.N <= 2048) {
+    if constexpr (EPI != SWIGLU_F32) {
+      if (KB > 32 && KB <= 64) return launch_few<1, 1, EPI, 16, 4, 8>(a, s);
     }
+    return launch_few<1, 1, EPI, 8, 2, 8>(a, s);
   }
   if constexpr (EPI != SWIGLU_F32) {
-    if (a.N <= 5120) return launch_few<WM, EPI, 16, 1, 16>(a, s);
+    if (a.N <= 5120) return launch_few<1, 1, EPI, 16, 1, 16>(a, s);
   }
-  return launch_few<WM, EPI, 8, 1, 16>(a, s);
+  return launch_few<1, 1, EPI, 8, 1, 16>(a, s);
 }
 
 template <int EPI>
-int few_rows(const Fp8Args& a, hipStream_t s) {
-  switch ((a.M + 15) / 16) {
-    case 1: return few_rows_as<1, EPI>(a, s);
-    case 2: return few_rows_as<2, EPI>(a, s);
-    case 3: return few_rows_as<3, EPI>(a, s);
-    default: return few_rows_as<4, EPI>(a, s);
+int by_strips(const Fp8Args& a, int shape, hipStream_t s) {
+  switch (shape) {
+    case 0: return launch_few<1, 1, EPI, 8, 1, 16>(a, s);
+    case 1: return launch_few<1, 2, EPI, 8, 1, 16>(a, s);
+    case 2: return launch_few<2, 1, EPI, 8, 1, 16>(a, s);
+    case 3: return launch_few<2, 2, EPI, 8, 1, 16>(a, s);
+    case 4: return launch_few<3, 2, EPI, 8, 1, 16>(a, s);
+    default: return launch_few<4, 2, EPI, 8, 1, 16>(a, s);
   }
 }
 
@@ -589,34 +596,27 @@ int launch_tiles(Fp8Args a, hipStream_t s) {
   return BW_LAUNCH_CHECK();
 }
 
-// What a shape of tile takes, in us: a workgroup's start and end, and a step of 128 of K, with the compute unit for itself and, where
-// two fit (``per_cu`` 2), beside another.  Measured on normal values (the power of the matrix cores, and with it their clock, hangs
-// on them): slopes over K = 2048 and 8192, grids of up to 256 workgroups and of one or two full rounds.
-struct TileCost {
+// What a workgroup of a shape (rows x columns) takes, in us: its start and end, and a step of 128 of K, with the compute unit for
+// itself and, where two fit (``per_cu`` 2), beside another.  Measured on normal values (the power of the matrix cores, and with it
+// their clock, hangs on them): slopes over K = 2048 and 8192, grids of up to 256 workgroups and of one or two full rounds.
+struct ShapeCost {
   int rows, columns, per_cu;
   double start, step, start_beside, step_beside;
 };
 
-double tiles_us(const TileCost& c, int M, int N, int K) {
+double shape_us(const ShapeCost& c, int M, int N, int K) {
   const double steps = K / BW_FP8_BLOCK, alone = c.start + steps * c.step, beside = c.start_beside + steps * c.step_beside;
-  const long long tiles = (long long)((M + c.rows - 1) / c.rows) * ((N + c.columns - 1) / c.columns);
-  const long long full = tiles / (256 * c.per_cu), rest = tiles % (256 * c.per_cu);
-  return 2.5 + full * (c.per_cu == 2 ? beside : alone) + (rest == 0 ? 0.0 : rest <= 256 ? alone : beside);
-}
-
-// Few rows: the matrix from memory (4.2 MB a us, the first byte included) and every strip's x from the L2s (7.2 MB a us), by as many units as there
-// are strips.
-double few_us(int M, int N, int K, int halves) {
-  const double strips = (N + 15) / 16, mb = 1e-6 * K * N;
-  return 1.5 + (mb * halves / 4.2 + 1e-6 * strips * M * K / 7.2) * (strips < 256 ? 256 / strips : 1.0);
+  const long long groups = (long long)((M + c.rows - 1) / c.rows) * ((N + c.columns - 1) / c.columns);
+  const long long full = groups / (256 * c.per_cu), rest = groups % (256 * c.per_cu);
+  return 2.0 + full * (c.per_cu == 2 ? beside : alone) + (rest == 0 ? 0.0 : rest <= 256 ? alone : beside);
 }
 
 template <int SHAPES>
-int cheapest(const TileCost (&shapes)[SHAPES], int M, int N, int K, double* us) {
+int cheapest(const ShapeCost (&shapes)[SHAPES], int M, int N, int K, double* us) {
   int best = 0;
-  *us = tiles_us(shapes[0], M, N, K);
+  *us = shape_us(shapes[0], M, N, K);
   for (int i = 1; i < SHAPES; ++i) {
-    const double t = tiles_us(shapes[i], M, N, K);
+    const double t = shape_us(shapes[i], M, N, K);
     if (t < *us) {
       *us = t;
       best = i;
@@ -625,10 +625,18 @@ int cheapest(const TileCost (&shapes)[SHAPES], int M, int N, int K, double* us) 
   return best;
 }
 
-// A step's conversions a matrix instruction fall with the tile: 192 x 256 a workgroup of eight waves does the most a us, 128 x 128 by
-// four waves, two workgroups a unit, fills a round sooner, 64 x 128 and 64 x 64 give a few hundred rows of few columns more workgroups.
-constexpr TileCost STORE_SHAPES[] = {{192, 256, 1, 6.0, 2.04, 0, 0}, {128, 128, 2, 5.3, 1.02, 6.0, 1.78}, {64, 128, 2, 2.4, 0.64, 2.6, 1.12}, {64, 64, 2, 2.0, 0.49, 2.7, 0.74}};
-constexpr TileCost GATED_SHAPES[] = {{192, 128, 1, 10.5, 2.04, 0, 0}, {128, 128, 1, 5.0, 1.70, 0, 0}, {64, 128, 2, 3.0, 1.20, 9.0, 1.60}, {32, 128, 2, 2.0, 0.95, 4.0, 1.30}};
+// Strips: each wave a block of K of its own, which hides what a tile's step waits for; x and the matrix come once a workgroup,
+// though, so many rows and columns are cheaper by tiles (64 x 4096 x 4096 11.2 us by strips, 19.5 by tiles; 40 x 28672 x 4096 49 and 30).
+constexpr ShapeCost STORE_STRIPS[] = {{16, 16, 2, 1.1, 0.115, 1.8, 0.19}, {16, 32, 2, 0.4, 0.173, 0.7, 0.285}, {32, 16, 2, 0.1, 0.20, 0.2, 0.33},
+                                      {32, 32, 2, 0.9, 0.27, 1.5, 0.445}, {48, 32, 1, 2.5, 0.29, 0, 0},        {64, 32, 1, 1.0, 0.44, 0, 0}};
+constexpr ShapeCost GATED_STRIPS[] = {{16, 16, 2, 0.4, 0.20, 0.7, 0.33}, {16, 32, 2, 0.5, 0.28, 0.9, 0.46}, {32, 16, 2, 0.0, 0.285, 0.0, 0.47},
+                                      {32, 32, 1, 0.6, 0.43, 0, 0},      {48, 32, 1, 1.0, 0.55, 0, 0},      {64, 32, 1, 1.0, 0.70, 0, 0}};
+// Tiles: a step's conversions a matrix instruction fall with the tile.  192 x 256 by eight waves does the most a us, 128 x 128 by four, two
+// workgroups a unit, fills a round sooner, 64 x 128 and 64 x 64 give a few hundred rows of few columns more workgroups.
+constexpr ShapeCost STORE_TILES[] = {{192, 256, 1, 6.5, 2.04, 0, 0}, {128, 128, 2, 5.8, 1.02, 6.5, 1.78}, {64, 128, 2, 2.9, 0.64, 3.1, 1.12}, {64, 64, 2, 2.5, 0.49, 3.2, 0.74}};
+constexpr ShapeCost GATED_TILES[] = {{192, 128, 1, 11.0, 2.04, 0, 0}, {128, 128, 1, 5.5, 1.70, 0, 0}, {64, 128, 2, 3.5, 1.20, 9.5, 1.60}, {32, 128, 2, 2.5, 0.95, 4.5, 1.30}};
+
+constexpr int STRIPS_MOST_ROWS = 1024;          // (the grid's second size stays small; far more rows are always cheaper by tiles)
 
 template <int EPI>
 int stored_by_tiles(const Fp8Args& a, int shape, hipStream_t s) {
@@ -651,7 +659,7 @@ int gated_by_tiles(const Fp8Args& a, int shape, hipStream_t s) {
 
 bool aligned(const void* p, int n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
-constexpr int FEW_ROWS = 64;
+constexpr int FEW_ROWS = 64;                    // rows up to which a gated product has a buffer for its sums
 
 // sizes that every entry point refuses
 int sizes_wrong(const void* x, int ldx, int ldxs, const void* w, int rows, int N, int K) {
@@ -675,9 +683,10 @@ extern "C" int bw_gemm_fp8(const void* x, int ldx, const float* xs, int ldxs, co
   a.vec_out = aligned(out, 16) && (rows == 1 || (long long)ldo * (out_is_bf16 ? 2 : 4) % 16 == 0) &&
               (residual == nullptr || (aligned(residual, 16) && (rows == 1 || ldr % 4 == 0)));
   hipStream_t s = (hipStream_t)stream;
-  double us;
-  const int shape = cheapest(STORE_SHAPES, rows, N, K, &us);
-  if (rows <= 16 || (rows <= FEW_ROWS && few_us(rows, N, K, 1) <= us)) return out_is_bf16 ? few_rows<STORE_BF16>(a, s) : few_rows<STORE_F32>(a, s);
+  if (rows <= 16) return out_is_bf16 ? sixteen_rows<STORE_BF16>(a, s) : sixteen_rows<STORE_F32>(a, s);
+  double us, strips_us;
+  const int shape = cheapest(STORE_TILES, rows, N, K, &us), strips = cheapest(STORE_STRIPS, rows, N, K, &strips_us);
+  if (rows <= STRIPS_MOST_ROWS && strips_us <= us) return out_is_bf16 ? by_strips<STORE_BF16>(a, strips, s) : by_strips<STORE_F32>(a, strips, s);
   return out_is_bf16 ? stored_by_tiles<STORE_BF16>(a, shape, s) : stored_by_tiles<STORE_F32>(a, shape, s);
 }
 
@@ -692,13 +701,13 @@ extern "C" int bw_gemm_fp8_swiglu(const void* x, int ldx, const float* xs, int l
   a.x = (const uint8_t*)x, a.xs = xs, a.w = (const uint8_t*)w, a.ws = ws;
   a.ldx = ldx, a.ldxs = ldxs, a.M = rows, a.N = inter, a.K = K;
   hipStream_t s = (hipStream_t)stream;
-  double us;
-  const int shape = cheapest(GATED_SHAPES, rows, inter, K, &us);
+  double us, strips_us;
+  const int shape = cheapest(GATED_TILES, rows, inter, K, &us), strips = cheapest(GATED_STRIPS, rows, inter, K, &strips_us);
   if (rows <= FEW_ROWS) {
     if (sums == nullptr || (rows > 1 && ldsums < inter)) return -2;
-    if (rows <= 16 || few_us(rows, inter, K, 2) + 2.5 <= us) {         // (the quantization of the sums is a launch of its own)
+    if (rows <= 16 || strips_us + 2.5 <= us) {                        // (the quantization of the sums is a launch of its own)
       a.out = sums, a.ldo = ldsums;
-      if (const int bad = few_rows<SWIGLU_F32>(a, s)) return bad;
+      if (const int bad = rows <= 16 ? sixteen_rows<SWIGLU_F32>(a, s) : by_strips<SWIGLU_F32>(a, strips, s)) return bad;
       return bw_quantize_fp8(sums, 0, ldsums, codes, ldq, scales, lds, rows, inter, stream);
     }
   }
