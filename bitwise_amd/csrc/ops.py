@@ -2043,32 +2043,40 @@ def _need_rows(t: torch.Tensor, dtype, what: str) -> None:
 # tensor's sizes and strides are asked for once, everything is looked at in one condition, and what is wrong is only worked out when
 # something is.  (A call with eleven checks as functions of their own took 8.5 us of the host's time, one so written 5.)
 
-def _matrix_arg(t: torch.Tensor, dtype, rows: int, width: int, device: int, what: str) -> Tuple[int, int]:
-    """A matrix [>= rows, width] on the device, rows contiguous and a stride apart: (pointer, stride; a single row's is its width)."""
-    if t.dtype is dtype and t.dim() == 2:
+_F32, _BF16 = torch.float32, torch.bfloat16
+
+
+def _matrix_arg(t: torch.Tensor, rows: int, width: int, device: int, what: str, f32_only: bool = False) -> Tuple[int, int, int]:
+    """A matrix [>= rows, width] on the device, rows contiguous and a stride apart: (pointer, stride, whether bfloat16); a single
+    row's stride is its width."""
+    dtype = t.dtype
+    if (dtype is _F32 or (dtype is _BF16 and not f32_only)) and t.dim() == 2:
         n, w = t.shape
         ld, inner = t.stride()
         if n >= rows and w == width and (inner == 1 or w == 1) and t.get_device() == device:
-            return t.data_ptr(), ld if rows > 1 else w
-    _need_rows(t, dtype, what)
+            return t.data_ptr(), ld if rows > 1 else w, dtype is _BF16
+    if dtype != _BF16 or f32_only:
+        _need_rows(t, _F32, what)
+    else:
+        _need_rows(t, _BF16, what)
     if t.shape[0] < rows or t.shape[1] != width:
         raise ValueError(f"{what} {tuple(t.shape)} does not fit {rows} rows of {width}")
     raise ValueError(f"{what}: all tensors live on the current device")
 
 
-def _vector_arg(t: Optional[torch.Tensor], dim: int, device: int, what: str) -> Tuple[Optional[int], int]:
-    """A vector [dim], bfloat16 or float32, or None: (pointer, whether bfloat16)."""
-    if t is None:
-        return None, 0
-    if t.dim() != 1 or t.shape[0] != dim or t.get_device() != device or not t.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous vector of {dim} on the current device, on the GPU")
-    return t.data_ptr(), _is_bf16(t, what)
+def _vector_arg(t: torch.Tensor, dim: int, device: int, what: str) -> Tuple[int, int]:
+    """A vector [dim], bfloat16 or float32: (pointer, whether bfloat16)."""
+    dtype = t.dtype
+    if (dtype is _F32 or dtype is _BF16) and t.dim() == 1 and t.numel() == dim and t.get_device() == device and t.is_contiguous():
+        return t.data_ptr(), dtype is _BF16
+    _is_bf16(t, what)
+    raise ValueError(f"{what} must be a contiguous vector of {dim} on the current device, on the GPU")
 
 
 def _codes_arg(codes: torch.Tensor, scales: torch.Tensor, rows: int, width: Optional[int], device: int, what: str) -> Tuple[int, int, int, int, int]:
     """Rows of codes [>= rows, whole blocks] e4m3 and their scales [blocks, >= rows] float32, the rows of both contiguous:
     (pointer, stride, scales' pointer, scales' stride from block to block, blocks)."""
-    if codes.dtype is FP8 and scales.dtype is torch.float32 and codes.dim() == 2 and scales.dim() == 2:
+    if codes.dtype is FP8 and scales.dtype is _F32 and codes.dim() == 2 and scales.dim() == 2:
         n, k = codes.shape
         blocks, r = scales.shape
         ld, inner = codes.stride()
@@ -2093,7 +2101,7 @@ def _codes_arg(codes: torch.Tensor, scales: torch.Tensor, rows: int, width: Opti
 
 def _fp8_matrix_arg(w: torch.Tensor, w_scales: torch.Tensor, halves: int, blocks: int, device: int, what: str) -> Tuple[int, int, int]:
     """A matrix [halves * N, blocks * 128] of codes with its scales: (pointer, scales' pointer, N)."""
-    if w.dtype is FP8 and w_scales.dtype is torch.float32 and w.dim() == 2 and w_scales.dim() == 2:
+    if w.dtype is FP8 and w_scales.dtype is _F32 and w.dim() == 2 and w_scales.dim() == 2:
         n, k = w.shape
         nb, kb = w_scales.shape
         if (n > 0 and n % halves == 0 and k == blocks * FP8_BLOCK and kb == blocks and nb == halves * (-(-(n // halves) // FP8_BLOCK))
@@ -2125,15 +2133,12 @@ def quantize_fp8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, row
 
     all in 32 bits, the codes rounded to nearest even.  ``codes`` [>= rows, fp8_width(K)] gets zeros behind the rows' end;
     ``scales`` [fp8_width(K) / 128, >= rows].  A block that holds an infinity or NaN stands for NaN throughout."""
-    dtype = x.dtype
-    if dtype is not torch.bfloat16 and dtype is not torch.float32:
-        raise ValueError(f"quantize_fp8: x must be bfloat16 or float32, got {dtype}")
-    if x.dim() != 2:
-        raise ValueError("quantize_fp8: x must be a matrix")
+    if x.dtype not in (_BF16, _F32) or x.dim() != 2:
+        raise ValueError(f"quantize_fp8: x must be a bfloat16 or float32 matrix, got {x.dtype}")
     device, width = _device_of(x, "quantize_fp8: x"), x.shape[1]
-    xp, ldx = _matrix_arg(x, dtype, rows, width, device, "quantize_fp8: x")
+    xp, ldx, xb = _matrix_arg(x, rows, width, device, "quantize_fp8: x")
     cp, ldc, sp, lds, _ = _codes_arg(codes, scales, rows, width, device, "quantize_fp8")
-    _check(_fn("bw_quantize_fp8")(xp, dtype is torch.bfloat16, ldx, cp, ldc, sp, lds, rows, width, _stream()), "quantize_fp8")
+    _check(_fn("bw_quantize_fp8")(xp, xb, ldx, cp, ldc, sp, lds, rows, width, _stream()), "quantize_fp8")
 
 
 def norm_add_norm(x: torch.Tensor, y: Optional[torch.Tensor], weight: torch.Tensor, out: torch.Tensor, rows: int, eps: float,
@@ -2152,38 +2157,38 @@ def norm_add_norm(x: torch.Tensor, y: Optional[torch.Tensor], weight: torch.Tens
     if x.dim() != 2:
         raise ValueError("norm_add_norm: x must be a matrix")
     device, dim = _device_of(x, "norm_add_norm: x"), x.shape[1]
-    xp, ldx = _matrix_arg(x, torch.float32, rows, dim, device, "norm_add_norm: x")
-    vector = isinstance(scale, torch.Tensor)
-    yp = yb = ldy = gp = gb = ldg = tp = ldt = 0
+    xp, ldx, _ = _matrix_arg(x, rows, dim, device, "norm_add_norm: x", True)
+    number = scale.__class__ is float or not isinstance(scale, torch.Tensor)
+    yp = yb = ldy = gp = gb = ldg = tp = ldt = pp = pb = vp = vb = cp = lds = 0
     if y is None:
-        if post_weight is not None or gate is not None or stream is not None or vector or scale != 1.0:
+        if post_weight is not None or gate is not None or stream is not None or not number or scale != 1.0:
             raise ValueError("norm_add_norm: without a sublayer's output there is nothing to norm, gate, scale or add")
     else:
-        yb = _is_bf16(y, "norm_add_norm: y")
-        yp, ldy = _matrix_arg(y, y.dtype, rows, dim, device, "norm_add_norm: y")
-        tp, ldt = (xp, ldx) if stream is None else _matrix_arg(stream, torch.float32, rows, dim, device, "norm_add_norm: stream")
-    if gate is not None:
-        if gate.dim() == 2:
-            gb = _is_bf16(gate, "norm_add_norm: gate")
-            gp, ldg = _matrix_arg(gate, gate.dtype, rows, dim, device, "norm_add_norm: gate")
-            if ldg == 0:
-                raise ValueError("norm_add_norm: a gate for all rows is a vector")
-        else:
-            gp, gb = _vector_arg(gate, dim, device, "norm_add_norm: gate")
-    cp, lds = 0, 0
+        yp, ldy, yb = _matrix_arg(y, rows, dim, device, "norm_add_norm: y")
+        tp, ldt = xp, ldx
+        if stream is not None:
+            tp, ldt, _ = _matrix_arg(stream, rows, dim, device, "norm_add_norm: stream", True)
+        if post_weight is not None:
+            pp, pb = _vector_arg(post_weight, dim, device, "norm_add_norm: post_weight")
+        if not number:
+            vp, vb = _vector_arg(scale, dim, device, "norm_add_norm: scale")
+        if gate is not None:
+            if gate.dim() == 2:
+                gp, ldg, gb = _matrix_arg(gate, rows, dim, device, "norm_add_norm: gate")
+                if ldg == 0:
+                    raise ValueError("norm_add_norm: a gate for all rows is a vector")
+            else:
+                gp, gb = _vector_arg(gate, dim, device, "norm_add_norm: gate")
     if (scales is not None) != (out.dtype is FP8):
         raise ValueError("norm_add_norm: codes come with scales, other rows without")
     if scales is not None:
         op, ldo, cp, lds, _ = _codes_arg(out, scales, rows, dim, device, "norm_add_norm")
         kind = 2
     else:
-        kind = _is_bf16(out, "norm_add_norm: out")
-        op, ldo = _matrix_arg(out, out.dtype, rows, dim, device, "norm_add_norm: out")
-    pp, pb = _vector_arg(post_weight, dim, device, "norm_add_norm: post_weight")
-    vp, vb = _vector_arg(scale if vector else None, dim, device, "norm_add_norm: scale")
+        op, ldo, kind = _matrix_arg(out, rows, dim, device, "norm_add_norm: out")
     wp, wb = _vector_arg(weight, dim, device, "norm_add_norm: weight")
     _check(_fn("bw_norm_add_norm")(xp, ldx, yp, yb, ldy, pp, pb, eps if post_eps is None else post_eps, gp, gb, ldg, bool(gate_sigmoid), vp, vb,
-                                   0.0 if vector else scale, tp, ldt, wp, wb, eps, op, kind, ldo, cp, lds, rows, dim, _stream()), "norm_add_norm")
+                                   scale if number else 0.0, tp, ldt, wp, wb, eps, op, kind, ldo, cp, lds, rows, dim, _stream()), "norm_add_norm")
 
 
 def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, rows: int,
@@ -2196,13 +2201,12 @@ def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales:
     device = _device_of(x, "gemm_fp8: x")
     xp, ldx, sp, lds, blocks = _codes_arg(x, x_scales, rows, None, device, "gemm_fp8")
     wp, wsp, n = _fp8_matrix_arg(w, w_scales, 1, blocks, device, "gemm_fp8")
-    bf16 = _is_bf16(out, "gemm_fp8: out")
-    op, ldo = _matrix_arg(out, out.dtype, rows, n, device, "gemm_fp8: out")
+    op, ldo, bf16 = _matrix_arg(out, rows, n, device, "gemm_fp8: out")
     rp = ldr = 0
     if residual is not None:
         if bf16:
             raise ValueError("gemm_fp8: what is added to a residual stays 32-bit")
-        rp, ldr = _matrix_arg(residual, torch.float32, rows, n, device, "gemm_fp8: residual")
+        rp, ldr, _ = _matrix_arg(residual, rows, n, device, "gemm_fp8: residual", True)
     _check(_fn("bw_gemm_fp8")(xp, ldx, sp, lds, wp, wsp, rp, ldr, op, ldo, bf16, rows, n, blocks * FP8_BLOCK, _stream()), "gemm_fp8")
 
 
@@ -2220,7 +2224,7 @@ def gemm_fp8_swiglu(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_
     if rows <= FP8_SUMS_ROWS:
         if sums is None:
             raise ValueError(f"gemm_fp8_swiglu: up to {FP8_SUMS_ROWS} rows need a buffer for their sums")
-        up, ldu = _matrix_arg(sums, torch.float32, rows, n, device, "gemm_fp8_swiglu: sums")
+        up, ldu, _ = _matrix_arg(sums, rows, n, device, "gemm_fp8_swiglu: sums", True)
     _check(_fn("bw_gemm_fp8_swiglu")(xp, ldx, sp, lds, wp, wsp, up, ldu, cp, ldc, osp, ldos, rows, n, blocks * FP8_BLOCK, _stream()), "gemm_fp8_swiglu")
 
 
