@@ -638,6 +638,48 @@ constexpr ShapeCost GATED_TILES[] = {{192, 128, 1, 11.0, 2.04, 0, 0}, {128, 128,
 
 constexpr int STRIPS_MOST_ROWS = 1024;          // (the grid's second size stays small; far more rows are always cheaper by tiles)
 
+constexpr int FEW_ROWS = 64;                    // rows up to which a gated product has a buffer for its sums
+
+// What runs: ``strips`` (of the tables above; SIXTEEN: up to 16 rows, the strips made for those), or -1 and ``tiles``, the last ``tail``
+// rows behind the tiles by strips of their own.
+constexpr int SIXTEEN = 100;
+struct Choice {
+  int strips, tiles, tail;
+};
+
+Choice choose_stored(int rows, int N, int K) {
+  if (rows <= 16) return {SIXTEEN, 0, 0};
+  double us, strips_us;
+  int shape = cheapest(STORE_TILES, rows, N, K, &us), tail = 0;
+  const int strips = cheapest(STORE_STRIPS, rows, N, K, &strips_us);
+  if (rows > STRIPS_MOST_ROWS) strips_us = us + 1.0;
+  // A few rows past whole tiles can cost a round of their own: then they go by strips, behind the tiles (777 x 5003 x 2000, of which 768
+  // rows are one round, 35.9 -> 32.7 us; 2100 x 2048 x 2048 31.5 -> 27.5).
+  double best = us < strips_us ? us : strips_us;
+  for (int i = 0; i < 4; ++i) {
+    const int rest = rows % STORE_TILES[i].rows;
+    if (rest == 0 || rest == rows || rest > FEW_ROWS) continue;
+    double rest_us;
+    cheapest(STORE_STRIPS, rest, N, K, &rest_us);
+    const double both = shape_us(STORE_TILES[i], rows - rest, N, K) + rest_us;
+    if (both < best) {
+      best = both;
+      tail = rest;
+      shape = i;
+    }
+  }
+  if (tail == 0 && strips_us <= us) return {strips, 0, 0};
+  return {-1, shape, tail};
+}
+
+Choice choose_gated(int rows, int inter, int K) {
+  if (rows <= 16) return {SIXTEEN, 0, 0};
+  double us, strips_us;
+  const int shape = cheapest(GATED_TILES, rows, inter, K, &us), strips = cheapest(GATED_STRIPS, rows, inter, K, &strips_us);
+  if (rows <= FEW_ROWS && strips_us + 2.5 <= us) return {strips, 0, 0};      // (the quantization of the sums is a launch of its own)
+  return {-1, shape, 0};
+}
+
 template <int EPI>
 int stored_by_tiles(const Fp8Args& a, int shape, hipStream_t s) {
   switch (shape) {
@@ -659,7 +701,6 @@ int gated_by_tiles(const Fp8Args& a, int shape, hipStream_t s) {
 
 bool aligned(const void* p, int n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
-constexpr int FEW_ROWS = 64;                    // rows up to which a gated product has a buffer for its sums
 
 // sizes that every entry point refuses
 int sizes_wrong(const void* x, int ldx, int ldxs, const void* w, int rows, int N, int K) {
@@ -683,37 +724,24 @@ extern "C" int bw_gemm_fp8(const void* x, int ldx, const float* xs, int ldxs, co
   a.vec_out = aligned(out, 16) && (rows == 1 || (long long)ldo * (out_is_bf16 ? 2 : 4) % 16 == 0) &&
               (residual == nullptr || (aligned(residual, 16) && (rows == 1 || ldr % 4 == 0)));
   hipStream_t s = (hipStream_t)stream;
-  if (rows <= 16) return out_is_bf16 ? sixteen_rows<STORE_BF16>(a, s) : sixteen_rows<STORE_F32>(a, s);
-  double us, strips_us;
-  int shape = cheapest(STORE_TILES, rows, N, K, &us);
-  const int strips = cheapest(STORE_STRIPS, rows, N, K, &strips_us);
-  if (rows > STRIPS_MOST_ROWS) strips_us = us + 1.0;
-  // A few rows past whole tiles can cost a round of their own: then they go by strips, behind the tiles (777 x 5003 x 2000, of which 768
-  // rows are one round, 35.9 -> 32.7 us; 2100 x 2048 x 2048 31.5 -> 27.5).
-  int tail = 0;
-  double best = us < strips_us ? us : strips_us;
-  for (int i = 0; i < 4; ++i) {
-    const int rest = rows % STORE_TILES[i].rows;
-    if (rest == 0 || rest == rows || rest > FEW_ROWS) continue;
-    double rest_us;
-    cheapest(STORE_STRIPS, rest, N, K, &rest_us);
-    const double both = shape_us(STORE_TILES[i], rows - rest, N, K) + rest_us;
-    if (both < best) {
-      best = both;
-      tail = rest;
-      shape = i;
-    }
-  }
-  if (tail > 0) {
-    a.M = rows - tail;
-    if (const int bad = out_is_bf16 ? stored_by_tiles<STORE_BF16>(a, shape, s) : stored_by_tiles<STORE_F32>(a, shape, s)) return bad;
-    const size_t head = rows - tail;
-    void* rest_out = out_is_bf16 ? (void*)((bf16_t*)out + head * ldo) : (void*)((float*)out + head * ldo);
-    return bw_gemm_fp8((const uint8_t*)x + head * ldx, ldx, xs + head, ldxs, w, ws, residual == nullptr ? nullptr : residual + head * ldr, ldr, rest_out, ldo,
-                       out_is_bf16, tail, N, K, stream);
-  }
-  if (strips_us <= us) return out_is_bf16 ? by_strips<STORE_BF16>(a, strips, s) : by_strips<STORE_F32>(a, strips, s);
-  return out_is_bf16 ? stored_by_tiles<STORE_BF16>(a, shape, s) : stored_by_tiles<STORE_F32>(a, shape, s);
+  const Choice c = choose_stored(rows, N, K);
+  if (c.strips == SIXTEEN) return out_is_bf16 ? sixteen_rows<STORE_BF16>(a, s) : sixteen_rows<STORE_F32>(a, s);
+  if (c.strips >= 0) return out_is_bf16 ? by_strips<STORE_BF16>(a, c.strips, s) : by_strips<STORE_F32>(a, c.strips, s);
+  a.M = rows - c.tail;
+  if (const int bad = out_is_bf16 ? stored_by_tiles<STORE_BF16>(a, c.tiles, s) : stored_by_tiles<STORE_F32>(a, c.tiles, s)) return bad;
+  if (c.tail == 0) return 0;
+  const size_t head = rows - c.tail;
+  void* rest_out = out_is_bf16 ? (void*)((bf16_t*)out + head * ldo) : (void*)((float*)out + head * ldo);
+  return bw_gemm_fp8((const uint8_t*)x + head * ldx, ldx, xs + head, ldxs, w, ws, residual == nullptr ? nullptr : residual + head * ldr, ldr, rest_out, ldo,
+                     out_is_bf16, c.tail, N, K, stream);
+}
+
+// Which kernels a product's sizes lead to (``Choice``): strips, tiles, tail.
+extern "C" int bw_gemm_fp8_choice(int rows, int N, int K, int gated, int* choice) {
+  if (rows < 1 || N < 1 || K < BW_FP8_BLOCK) return -2;
+  const Choice c = gated ? choose_gated(rows, N, K) : choose_stored(rows, N, K);
+  choice[0] = c.strips, choice[1] = c.tiles, choice[2] = c.tail;
+  return 0;
 }
 
 extern "C" int bw_gemm_fp8_swiglu(const void* x, int ldx, const float* xs, int ldxs, const void* w, const float* ws, float* sums, int ldsums, void* codes,
@@ -727,16 +755,13 @@ extern "C" int bw_gemm_fp8_swiglu(const void* x, int ldx, const float* xs, int l
   a.x = (const uint8_t*)x, a.xs = xs, a.w = (const uint8_t*)w, a.ws = ws;
   a.ldx = ldx, a.ldxs = ldxs, a.M = rows, a.N = inter, a.K = K;
   hipStream_t s = (hipStream_t)stream;
-  double us, strips_us;
-  const int shape = cheapest(GATED_TILES, rows, inter, K, &us), strips = cheapest(GATED_STRIPS, rows, inter, K, &strips_us);
-  if (rows <= FEW_ROWS) {
-    if (sums == nullptr || (rows > 1 && ldsums < inter)) return -2;
-    if (rows <= 16 || strips_us + 2.5 <= us) {                        // (the quantization of the sums is a launch of its own)
-      a.out = sums, a.ldo = ldsums;
-      if (const int bad = rows <= 16 ? sixteen_rows<SWIGLU_F32>(a, s) : by_strips<SWIGLU_F32>(a, strips, s)) return bad;
-      return bw_quantize_fp8(sums, 0, ldsums, codes, ldq, scales, lds, rows, inter, stream);
-    }
+  const Choice c = choose_gated(rows, inter, K);
+  if (rows <= FEW_ROWS && (sums == nullptr || (rows > 1 && ldsums < inter))) return -2;
+  if (c.strips >= 0) {
+    a.out = sums, a.ldo = ldsums;
+    if (const int bad = c.strips == SIXTEEN ? sixteen_rows<SWIGLU_F32>(a, s) : by_strips<SWIGLU_F32>(a, c.strips, s)) return bad;
+    return bw_quantize_fp8(sums, 0, ldsums, codes, ldq, scales, lds, rows, inter, stream);
   }
   a.out = codes, a.ldo = ldq, a.out_scales = scales, a.lds = lds;
-  return gated_by_tiles(a, shape, s);
+  return gated_by_tiles(a, c.tiles, s);
 }

@@ -168,6 +168,7 @@ _SIGS = {
                          c_float, c_void_p, c_int, c_void_p, c_int, c_float, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_void_p],
     "bw_gemm_fp8": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int,
                     c_void_p],
+    "bw_gemm_fp8_choice": [c_int, c_int, c_int, c_int, c_void_p],
     "bw_gemm_fp8_swiglu": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int,
                            c_int, c_int, c_void_p],
 }
@@ -184,7 +185,7 @@ _CHAIN_KEEPS = frozenset({
     "bw_gemm_gelu_glu_wins", "bw_gemm_split_tile", "bw_gemm_split_rows", "bw_attention_f32_waves", "bw_fingerprint_waves",
     "bw_gemm_add_scratch", "bw_norm_gemm_supported", "bw_norm_gemm_wide_supported", "bw_norm_gemm_strips", "bw_attention_decode_scratch",
     "bw_attention_fold_group_tiles", "bw_gemm_add_bf16_static_max", "bw_moe_max_tiles", "bw_shared_key_piece", "bw_chain_sync_words", "bw_chain_begin",
-    "bw_chain_flush", "bw_chain_end",
+    "bw_chain_flush", "bw_chain_end", "bw_gemm_fp8_choice",
 })
 _chain_open = False
 
@@ -2208,6 +2209,14 @@ def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales:
             raise ValueError("gemm_fp8: what is added to a residual stays 32-bit")
         rp, ldr, _ = _matrix_arg(residual, rows, n, device, "gemm_fp8: residual", True)
     _check(_fn("bw_gemm_fp8")(xp, ldx, sp, lds, wp, wsp, rp, ldr, op, ldo, bf16, rows, n, blocks * FP8_BLOCK, _stream()), "gemm_fp8")
+
+
+def gemm_fp8_choice(rows: int, n: int, k: int, gated: bool = False) -> Tuple[int, int, int]:
+    """Which kernels a product of these sizes (``k`` in whole blocks) runs, see gemm_fp8.hip: (strips, or -1; tiles; rows behind the
+    tiles that go by strips)."""
+    out = (c_int * 3)()
+    _check(_fn("bw_gemm_fp8_choice")(int(rows), int(n), int(k), int(gated), ctypes.cast(out, c_void_p)), "gemm_fp8_choice")
+    return tuple(out)
 
 
 def gemm_fp8_swiglu(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, codes: torch.Tensor,

@@ -215,8 +215,9 @@ extern "C" int bw_norm_add_norm(const float* x, int ldx, const void* y, int y_is
                                 float* stream_out, int ldst, const void* weight, int weight_is_bf16, float eps, void* out, int out_kind, int ldo,
                                 float* scales, int lds, int rows, int dim, void* stream) {
   if (rows <= 0) return 0;
-  if (dim < 1 || dim > 0x7ffff000 || out_kind < 0 || out_kind > 2 || (y != nullptr && stream_out == nullptr) || (out_kind == OUT_FP8 && (scales == nullptr || lds < rows)))
+  if (dim < 1 || dim > 0x7ffff000 || rows > (1 << 21) || out_kind < 0 || out_kind > 2 || (y != nullptr && stream_out == nullptr) || (out_kind == OUT_FP8 && (scales == nullptr || lds < rows)))
     return -2;
+  if (y != nullptr && out == stream_out) return -2;              // (two results, one place)
   if (y == nullptr && (post_weight != nullptr || gate != nullptr || scale_vec != nullptr)) return -2;
   if (out_kind == OUT_FP8 && (!aligned16(out) || ldo % 16)) return -3;
   NormAddNormArgs a;

@@ -93,7 +93,7 @@ __device__ __forceinline__ uint32_t largest8(const float (&v)[8]) {
 
 // 1 / (1 + exp(-g)) within two units in the last place: codes are rounded from it, and what is more off moves more of them to
 // a neighbour.  The exponential through the hardware exp2, its argument in two parts; the quotient through the hardware
-// reciprocal and one Newton step.  (Below -88 the argument stays there: the result is under 10^-38.)  NaN gives a number.
+// reciprocal and one Newton step.  (Below -88 the argument stays there: silu is off by less than 10^-36.)  NaN gives a number.
 __device__ __forceinline__ float sigmoid_of_number(float g) {
   const float x = fminf(-g, 88.0f);
   const float hi = x * 0x1.715476p+0f;

@@ -461,3 +461,115 @@ def test_offsets_past_31_bits(gpu):
     ops.quantize_fp8(big, codes, scales, rows)
     want_c, want_s = quantized(tail)
     assert same_bits(codes[-8:].contiguous(), want_c) and same_bits(scales[:, -8:].contiguous(), want_s)
+
+
+# ------------------------------------------------------------------------------ every kernel that sizes lead to
+
+# one block of K, and several: every strip and tile, plain and gated, and tiles with rows behind them (tests/test_fp8_rules.py checks
+# that these sizes reach them all)
+STORED = [(17, 68, 1792), (19, 77, 1536), (17, 70, 128), (18, 4904, 1792), (33, 6155, 1280), (34, 6328, 384), (335, 21916, 128), (199, 25401, 128),
+          (3348, 261, 128), (1068, 65, 128), (400, 23971, 128), (194, 16868, 128), (1295, 1544, 1920), (960, 4391, 1280),
+          (257, 22075, 640), (1001, 4090, 1152), (310, 6005, 1152), (500, 1501, 1152), (60, 6300, 1152)]
+GATED = [(17, 66, 640), (35, 2069, 384), (17, 67, 128), (17, 4591, 2176), (33, 6263, 384), (49, 6714, 640), (137, 27323, 128), (68, 22010, 128),
+         (33, 20016, 128), (68, 65, 128), (132, 22012, 640), (67, 22083, 640), (33, 16470, 640), (200, 5003, 1152), (90, 1501, 1152)]
+
+
+def on_gpu(codes, scales, halves=1):
+    """A matrix's values in 64 bits, on the GPU."""
+    n, nb = codes.shape[0] // halves, scales.shape[0] // halves
+    at = torch.arange(n, device=codes.device) // 128
+    at = torch.cat([at + h * nb for h in range(halves)])
+    return codes.double() * scales.double()[at][:, torch.arange(codes.shape[1], device=codes.device) // 128]
+
+
+@pytest.mark.parametrize("rows,n,k", STORED, ids=lambda v: str(v))
+def test_every_strip_and_tile(gpu, rows, n, k):
+    x, xs, x64 = rows_of_codes(rows, k, rows, gpu)
+    w, ws, _ = matrix(n, k, n, gpu)
+    x64, w64 = x64.to(gpu), on_gpu(w, ws)
+    want = torch.mm(x64, w64.t().contiguous())
+    bound = (128 + 2 * k // 128 + 2) * U * torch.mm(x64.abs(), w64.abs().t().contiguous()) + 1e-40
+    out = torch.full((rows + 1, n), 9.0, device=gpu)
+    ops.gemm_fp8(x, xs, w, ws, out, rows)
+    assert ((out[:rows].double() - want).abs() <= bound).all() and (out[rows] == 9.0).all()
+    rounded = torch.full((rows + 1, n + 8), 9.0, device=gpu, dtype=torch.bfloat16)
+    ops.gemm_fp8(x, xs, w, ws, rounded[:, :n], rows)
+    assert same_bits(rounded[:rows, :n].contiguous(), out[:rows].bfloat16()) and (rounded[rows] == 9.0).all() and (rounded[:, n:] == 9.0).all()
+    residual = torch.randn(rows, n, generator=gen(5)).to(gpu) * want.abs().mean().item()
+    added = residual.clone()
+    ops.gemm_fp8(x, xs, w, ws, added, rows, residual=added)
+    assert same_bits(added, residual + out[:rows])
+    # the bits of every row hang on the row alone: the last ones by themselves
+    last = torch.empty(min(rows, 16), n, device=gpu)
+    first = rows - last.shape[0]
+    ops.gemm_fp8(x[first:], xs[:, first:], w, ws, last, last.shape[0])
+    assert same_bits(last, out[first:rows])
+
+
+@pytest.mark.parametrize("rows,inter,k", GATED, ids=lambda v: str(v))
+def test_every_gated_strip_and_tile(gpu, rows, inter, k):
+    x, xs, _ = rows_of_codes(rows, k, rows, gpu)
+    w, ws, _ = matrix(inter, k, inter, gpu, halves=2, size=0.1)
+    codes, scales = codes_like(rows, inter, gpu, more=1)
+    ops.gemm_fp8_swiglu(x, xs, w, ws, codes, scales, rows, sums=torch.empty(64, inter, device=gpu))
+    assert (codes[rows].view(torch.uint8) == 0x2a).all() and (scales[:, rows] == 7.0).all()
+    # the two products' own sums, whose bits the tests above check: silu(g) u of them in 64 bits, then the definition of the codes
+    half = ws.shape[0] // 2
+    g, u = torch.empty(rows, inter, device=gpu), torch.empty(rows, inter, device=gpu)
+    ops.gemm_fp8(x, xs, w[:inter].contiguous(), ws[:half].contiguous(), g, rows)
+    ops.gemm_fp8(x, xs, w[inter:].contiguous(), ws[half:].contiguous(), u, rows)
+    want = g.double() * torch.sigmoid(g.double()) * u.double()
+    near = 8 * U * want.abs() + 1e-36                              # the sigmoid's four steps, two products
+    spread = scales[:, :rows].double().t().repeat_interleave(128, 1)
+    got = (codes[:rows].double() * spread)[:, :inter]
+    allowed = near * (1 + 2.0 ** -4) + torch.maximum(want.abs() * 2.0 ** -4, spread[:, :inter] * 2.0 ** -10) + 4 * U * want.abs()
+    assert ((got - want).abs() <= allowed).all()
+    pad = lambda t: torch.nn.functional.pad(t, (0, ops.fp8_width(inter) - inter)).view(rows, -1, 128).amax(dim=2)
+    assert ((scales[:, :rows].double().t() * 448 - pad(want.abs())).abs() <= pad(near) + 2 * U * pad(want.abs()) + 449 * TINY).all()
+    few = min(rows, 16)
+    last_c, last_s = codes_like(few, inter, gpu)
+    ops.gemm_fp8_swiglu(x[rows - few:], xs[:, rows - few:], w, ws, last_c, last_s, few, sums=torch.empty(16, inter, device=gpu))
+    assert same_bits(last_c, codes[rows - few:rows]) and same_bits(last_s, scales[:, rows - few:rows].contiguous())
+
+
+def test_two_results_in_one_place_are_refused(gpu):
+    x, y, w = torch.randn(4, 256, device=gpu), torch.randn(4, 256, device=gpu), torch.ones(256, device=gpu)
+    before = x.clone()
+    with pytest.raises(RuntimeError, match="norm_add_norm"):
+        ops.norm_add_norm(x, y, w, x, 4, 1e-6)
+    assert same_bits(x, before)
+
+
+def test_wrappers_refuse_what_does_not_fit(gpu):
+    x, c, s = torch.randn(4, 300, device=gpu), *codes_like(4, 300, gpu)
+    w, ws, _ = matrix(70, 300, 1, gpu)
+    out = torch.empty(4, 70, device=gpu)
+    for call, says in (
+            (lambda: ops.quantize_fp8(x, c[:, :256], s[:2], 4), "codes of rows of 300"),
+            (lambda: ops.quantize_fp8(x, c, s[:, :3], 4), "do not fit"),
+            (lambda: ops.quantize_fp8(x[:3], c, s, 4), "does not fit"),
+            (lambda: ops.quantize_fp8(x.t(), c, s, 4), "rows are contiguous"),
+            (lambda: ops.quantize_fp8(x, c.view(torch.uint8), s, 4), "float8"),
+            (lambda: ops.quantize_fp8(x, c, s.double(), 4), "float32"),
+            (lambda: ops.gemm_fp8(c[:, :200], s, w, ws, out, 4), "whole blocks"),
+            (lambda: ops.gemm_fp8(c, s, w[:, :256].contiguous(), ws[:, :2].contiguous(), out, 4), "does not fit"),
+            (lambda: ops.gemm_fp8(c, s, w, ws[:, :2], out, 4), "does not fit"),
+            (lambda: ops.gemm_fp8(c, s, w, ws, out[:, :60], 4), "does not fit"),
+            (lambda: ops.gemm_fp8(c, s, w, ws, out[:2], 4), "does not fit"),
+            (lambda: ops.gemm_fp8(c, s, w, ws, out.bfloat16(), 4, residual=out), "stays 32-bit"),
+            (lambda: ops.gemm_fp8(c, s, w, ws, out, 4, residual=out.double()), "float32"),
+            (lambda: ops.gemm_fp8(c[:, 8:], s, w, ws, out, 4), "whole blocks"),
+            (lambda: ops.gemm_fp8_swiglu(c, s, w, ws, *codes_like(4, 35, gpu), 4), "scales"),
+            (lambda: ops.norm_add_norm(x, None, x[0], c, 4, 1e-6), "codes come with scales"),
+            (lambda: ops.norm_add_norm(x, None, x[0], out, 4, 1e-6, scales=s), "codes come with scales"),
+            (lambda: ops.norm_add_norm(x, None, x[0], x.clone(), 4, 1e-6, gate=x), "nothing to norm"),
+            (lambda: ops.norm_add_norm(x, x[:2], x[0], x.clone(), 4, 1e-6), "does not fit"),
+            (lambda: ops.norm_add_norm(x, x.half(), x[0], x.clone(), 4, 1e-6), "float32"),
+            (lambda: ops.norm_add_norm(x, x, x[0, :200], x.clone(), 4, 1e-6), "vector of 300"),
+            (lambda: ops.norm_add_norm(x, x, x[0], x.clone(), 4, 1e-6, gate=x[0].expand(4, 300)), "a vector"),
+            (lambda: ops.norm_add_norm(x, x, x[0], x.clone(), 4, 1e-6, scale=x[:, 0]), "vector of 300")):
+        with pytest.raises(ValueError, match=says):
+            call()
+    w2, ws2, _ = matrix(40, 300, 2, gpu, halves=2)
+    with pytest.raises(ValueError, match="buffer for their sums"):
+        ops.gemm_fp8_swiglu(c, s, w2, ws2, *codes_like(4, 40, gpu), 4)

@@ -22,7 +22,7 @@ def test_quantization_refuses():
     assert quantize(rows=2 ** 21, lds=2 ** 21) == -2
 
 
-def norm(x=P, y=P, post=None, gate=None, ldg=0, vec=None, stream=P, out=P, kind=0, ldo=256, scales=None, lds=0, rows=4, dim=256):
+def norm(x=P, y=P, post=None, gate=None, ldg=0, vec=None, stream=P, out=2 * P, kind=0, ldo=256, scales=None, lds=0, rows=4, dim=256):
     return ops._fn("bw_norm_add_norm")(x, 256, y, 0, 256, post, 0, 1e-6, gate, 0, ldg, 0, vec, 0, 1.0, stream, 256, P, 0, 1e-6, out, kind, ldo, scales, lds,
                                        rows, dim, None)
 
@@ -30,8 +30,9 @@ def norm(x=P, y=P, post=None, gate=None, ldg=0, vec=None, stream=P, out=P, kind=
 def test_norm_refuses():
     assert norm(rows=0) == 0
     assert norm(dim=0) == -2 and norm(kind=3) == -2 and norm(stream=None) == -2
+    assert norm(out=P) == -2                                                          # both results in one place
     assert norm(kind=2) == -2 and norm(kind=2, scales=P, lds=3) == -2                 # codes without scales, or with too few
-    assert norm(kind=2, scales=P, lds=4, out=P + 4) == -3 and norm(kind=2, scales=P, lds=4, ldo=260) == -3
+    assert norm(kind=2, scales=P, lds=4, out=2 * P + 4) == -3 and norm(kind=2, scales=P, lds=4, ldo=260) == -3
     for given in ("post", "gate", "vec"):
         assert norm(y=None, **{given: P}) == -2                                       # nothing to norm, gate or scale
 
@@ -74,3 +75,21 @@ def test_wrappers_refuse_tensors_off_the_gpu():
 
 def test_width_of_rows_of_codes():
     assert [ops.fp8_width(n) for n in (1, 127, 128, 129, 2000)] == [128, 128, 128, 256, 2048]
+
+
+def test_the_gpu_tests_sizes_reach_every_kernel():
+    import test_fp8_gpu as sizes
+
+    stored = [ops.gemm_fp8_choice(rows, n, ops.fp8_width(k)) for rows, n, k in sizes.STORED]
+    assert {c[0] for c in stored} - {-1} == set(range(6)) and {c[1] for c in stored if c[0] < 0 and not c[2]} == set(range(4))
+    assert len({c[1] for c in stored if c[2]}) >= 3
+    long = [ops.gemm_fp8_choice(rows, n, ops.fp8_width(k)) for rows, n, k in sizes.STORED if k > 512]
+    assert {c[1] for c in long if c[0] < 0} == set(range(4))
+    gated = [ops.gemm_fp8_choice(rows, n, ops.fp8_width(k), gated=True) for rows, n, k in sizes.GATED]
+    assert {c[0] for c in gated} - {-1} == set(range(6)) and {c[1] for c in gated if c[0] < 0} == set(range(4))
+    long = [ops.gemm_fp8_choice(rows, n, ops.fp8_width(k), gated=True) for rows, n, k in sizes.GATED if k > 512]
+    assert {c[1] for c in long if c[0] < 0} == set(range(4))
+    for n, k in ((2048, 2048), (2048, 8192), (4096, 4096), (6144, 4096)):
+        assert ops.gemm_fp8_choice(16, n, k)[0] == 100 and ops.gemm_fp8_choice(17, n, k)[0] != 100
+    with pytest.raises(RuntimeError):
+        ops.gemm_fp8_choice(0, 64, 128)
