@@ -557,9 +557,10 @@ int launch_few(const Fp8Args& a, hipStream_t s) {
 
 // Up to 16 rows: strips of 16 columns for the 256 compute units, K's blocks over the waves of one.  Eight waves a strip where there are
 // strips for more than one workgroup a unit (8 rows of 28672 columns, K = 4096: 27.0 us, with 16 waves 28.2), 16 where there is about
-// one (4096 columns, K = 8192: 10.4, with eight 10.8).  Up to 2048 columns strips of eight, so that every unit has one: of 2048 columns,
-// K = 2048, 3.4 us for 3.7; K = 8192 with all of K asked for at once by 16 waves 8.3 for 9.8, with eight waves 9.0 (K = 2048 so 5.8:
-// most waves have nothing).
+// one (4096 columns, K = 8192: 10.4, with eight 10.8).  Two strips a workgroup, which halves what x costs, where there are more still
+// and x counts (16 rows of 28672 columns 31.8 -> 29.4 us, 8 of 6144 9.3 -> 8.3, gated 8 x 8192 x 2048 12.4 -> 11.9; but 2 x 16384 x 8192
+// 28.0 -> 31.5).  Up to 2048 columns strips of eight, so that every unit has one: of 2048 columns, K = 2048, 3.4 us for 3.7; K = 8192
+// with all of K asked for at once by 16 waves 8.3 for 9.8, with eight waves 9.0 (K = 2048 so 5.8: most waves have nothing).
 template <int EPI>
 int sixteen_rows(const Fp8Args& a, hipStream_t s) {
   const int KB = a.K / BW_FP8_BLOCK;
@@ -572,6 +573,7 @@ int sixteen_rows(const Fp8Args& a, hipStream_t s) {
   if constexpr (EPI != SWIGLU_F32) {
     if (a.N <= 5120) return launch_few<1, 1, EPI, 16, 1, 16>(a, s);
   }
+  if (a.N > 5120 && (EPI == SWIGLU_F32 || a.M > 4)) return launch_few<1, 2, EPI, 8, 1, 16>(a, s);
   return launch_few<1, 1, EPI, 8, 1, 16>(a, s);
 }
 
