@@ -81,10 +81,10 @@ class LlamaConfig:
             if d.get(key):
                 raise ConfigError(f"{key}=true is not supported by the Llama parts of this engine")
         quantized = d.get("quantization_config")
-        if quantized and (quantized.get("quant_method") != "fp8" or quantized.get("fmt", "e4m3") != "e4m3"
+        if quantized and (not isinstance(quantized, Mapping) or quantized.get("quant_method") != "fp8" or quantized.get("fmt", "e4m3") != "e4m3"
                           or quantized.get("activation_scheme", "dynamic") != "dynamic" or list(quantized.get("weight_block_size") or []) != [128, 128]):
             raise ConfigError("quantization_config: matrices in 8 bits are e4m3 codes with a scale for each block of 128 x 128 (quant_method "
-                              f"'fp8', weight_block_size [128, 128], inputs quantized as they come), got {dict(quantized)}")
+                              f"'fp8', weight_block_size [128, 128], inputs quantized as they come), got {quantized}")
         act = d.get("hidden_act", "silu")
         if act != "silu":
             raise ConfigError(f"hidden_act '{act}' is not supported; the feed-forward is SwiGLU with SiLU")

@@ -99,6 +99,8 @@ __device__ __forceinline__ void store_one(const Fp8Args& a, int m, int n, float 
 // K go round the waves, D to a wave and pass, all asked for before any is waited for; their sums meet in LDS, where the threads that
 // own the outputs walk them in order.  CW = 8 halves a strip (lanes with r >= 8 ask for nothing): twice as many workgroups, for
 // products with too few columns to give every compute unit 16.  More strips a workgroup share x's loads and its conversion.
+// Bound by the matrix's bytes and, at a few us, by what is not overlapped with them: 8 rows of 6144 columns, K = 4096, 7.8 us of
+// which loading alone takes 6 to 6.7, x 0.7 to 1.5, the walk 0.2 to 0.6 (a launch's start and end are 2); 28672 columns 27 us, 4.4 TB/s.
 template <int WM, int NC, int EPI, int NW, int D, int CW>
 __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
   constexpr int NB = EPI == SWIGLU_F32 ? 2 : 1, NS = NB * NC;                    // (strip c of gate or up b: c * NB + b)
@@ -219,11 +221,17 @@ __device__ __forceinline__ float taken(float v) {
   return r;
 }
 
-// A workgroup of eight waves computes BM rows times BN matrix rows (gated: BN / 2 gate and BN / 2 up rows) in steps of one
-// block of 128; both operands travel from memory straight into LDS, some steps ahead.  The waves lie WY x 8 / WY over the tile,
-// each with MI x NJ results of 16 x 16.  One load of a wave brings 8 rows of a step, 128 bytes each, into 1 KB of LDS, lane l's 16
+// A workgroup computes BM rows times BN matrix rows (gated: BN / 2 gate and BN / 2 up rows) in steps of one block of 128; both
+// operands travel from memory straight into LDS, ST steps ahead.  The waves lie WY x WAVES / WY over the tile, each with MI x NJ
+// results of 16 x 16.  One load of a wave brings 8 rows of a step, 128 bytes each, into 1 KB of LDS, lane l's 16
 // bytes to 16 l; slot c' of row r (within its block of 16 rows) holds the row's chunk c' ^ (r >> 1), so that the 16 lanes that
-// read one chunk of 16 rows hit 16 different groups of banks.
+// read one chunk of 16 rows hit 16 different groups of banks (conflicts: 1 % of LDS's busy cycles).
+//
+// What bounds it, of 2048 rows by gated 14336 columns, K = 4096, 404 us (1.19 PFLOP/s; a plain bfloat16 product of the library reaches
+// 1.38): the matrix cores are busy 52 % of the cycles, and for 16 matrix instructions of a wave there are 55 others, of which 27 convert
+// and 18 join chains.  Left out one at a time the conversions are worth 11 %, three quarters of the chains' multiply-adds 8 %, the reads
+// from LDS 9 %, all three together 24 %: then the clock falls with the matrix cores' power (zeros for operands run 8 % faster).  So the
+// tile is as large as a wave's registers allow: a step of 192 x 256 takes 2.04 us, of 128 x 128 for the same work 2.7.
 template <int EPI, int WAVES_, int WY_, int MI_, int NJ_, int ST_>
 struct Fp8Tile {
   static constexpr int WAVES = WAVES_, WY = WY_, WX = WAVES / WY_, MI = MI_, NJ = NJ_, ST = ST_;
@@ -382,8 +390,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
         }
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-          constexpr int at = 0;
-          f32x4& pj = p[PN == 1 ? at : i & 1][j];
+          f32x4& pj = p[PN == 1 ? 0 : i & 1][j];
           if (PN == 1 && t == 0) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) add_up((i + MI - 1) % MI, 4 * j + q);
@@ -476,7 +483,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
       if (g == 0) most[wx * BM + 16 * (MI * wy + i) + r] = mx;
     }
     __syncthreads();
-// The codes of the tile's rows lie in LDS row by row (144 bytes apart, which spreads the columns' words over the banks) and
+    // The codes of the tile's rows lie in LDS row by row (144 bytes apart, which spreads the columns' words over the banks) and
     // leave as whole lines.
     constexpr int CODES_AT = 4 * T::WX * BM, CLD = 144;
 #pragma unroll
@@ -703,7 +710,6 @@ int gated_by_tiles(const Fp8Args& a, int shape, hipStream_t s) {
 
 bool aligned(const void* p, int n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
-
 // sizes that every entry point refuses
 int sizes_wrong(const void* x, int ldx, int ldxs, const void* w, int rows, int N, int K) {
   if (N < 1 || K < BW_FP8_BLOCK || K % BW_FP8_BLOCK || K > (1 << 22) || N > (1 << 24) || rows > (1 << 22) || (rows > 1 && ldx < K) || ldxs < rows) return -2;
@@ -719,7 +725,7 @@ extern "C" int bw_gemm_fp8(const void* x, int ldx, const float* xs, int ldxs, co
   if (rows <= 0) return 0;
   if (const int bad = sizes_wrong(x, ldx, ldxs, w, rows, N, K)) return bad;
   if (rows > 1 && (ldo < N || (residual != nullptr && ldr < N))) return -2;
-  if (out_is_bf16 && residual != nullptr) return -2;
+  if ((out_is_bf16 && residual != nullptr) || out == x) return -2;                    // (x: other workgroups still read it)
   Fp8Args a = {};
   a.x = (const uint8_t*)x, a.xs = xs, a.w = (const uint8_t*)w, a.ws = ws, a.residual = residual, a.out = out;
   a.ldx = ldx, a.ldxs = ldxs, a.ldr = ldr, a.ldo = ldo, a.M = rows, a.N = N, a.K = K;
@@ -751,7 +757,7 @@ extern "C" int bw_gemm_fp8_swiglu(const void* x, int ldx, const float* xs, int l
   if (rows <= 0) return 0;
   if (const int bad = sizes_wrong(x, ldx, ldxs, w, rows, inter, K)) return bad;
   const int whole = (inter + BW_FP8_BLOCK - 1) / BW_FP8_BLOCK * BW_FP8_BLOCK;
-  if ((rows > 1 && ldq < whole) || lds < rows) return -2;
+  if ((rows > 1 && ldq < whole) || lds < rows || codes == x || scales == xs) return -2;   // (x: other workgroups still read it)
   if (!aligned(codes, 16) || ldq % 16) return -3;
   Fp8Args a = {};
   a.x = (const uint8_t*)x, a.xs = xs, a.w = (const uint8_t*)w, a.ws = ws;

@@ -2133,7 +2133,8 @@ def quantize_fp8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, row
         scales[b, r] = max(max |x[r, block b]|, 448 * 2^-126) / 448,  codes[r, k] = e4m3(x[r, k] * (1 / scales[b, r]))
 
     all in 32 bits, the codes rounded to nearest even.  ``codes`` [>= rows, fp8_width(K)] gets zeros behind the rows' end;
-    ``scales`` [fp8_width(K) / 128, >= rows].  A block that holds an infinity or NaN stands for NaN throughout."""
+    ``scales`` [fp8_width(K) / 128, >= rows].  A block that holds an infinity or NaN stands for NaN throughout.
+    ``codes`` is memory of its own."""
     if x.dtype not in (_BF16, _F32) or x.dim() != 2:
         raise ValueError(f"quantize_fp8: x must be a bfloat16 or float32 matrix, got {x.dtype}")
     device, width = _device_of(x, "quantize_fp8: x"), x.shape[1]
@@ -2198,7 +2199,8 @@ def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales:
     ``w`` [N, fp8_width(K)] with zeros behind K and ``w_scales`` [ceil(N / 128), fp8_width(K) / 128], a scale for each 128 x 128
     block.  Each block's products are summed in 32 bits, the blocks' sums times their two scales are added up in 32 bits, k
     ascending: a row's bits do not depend on the rows beside it.  ``out`` is float32 or bfloat16 (one rounding), its rows a stride
-    apart; ``residual`` (float32, with a float32 ``out``, which it may be) is added last."""
+    apart; ``residual`` (float32, with a float32 ``out``, which it may be) is added last.  ``out`` shares no memory with
+    ``x``."""
     device = _device_of(x, "gemm_fp8: x")
     xp, ldx, sp, lds, blocks = _codes_arg(x, x_scales, rows, None, device, "gemm_fp8")
     wp, wsp, n = _fp8_matrix_arg(w, w_scales, 1, blocks, device, "gemm_fp8")
@@ -2224,7 +2226,8 @@ def gemm_fp8_swiglu(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_
     """codes, scales [:rows] = ``quantize_fp8`` of silu(g) * u with [g | u] = x @ w.T as ``gemm_fp8`` computes it: a feed-forward's first half,
     ready for the product with its down projection.  ``w`` [2N, K] holds the gate rows, then the up rows, each half with scale
     blocks of its own: ``w_scales`` [2 ceil(N / 128), K / 128].  More than 64 rows: one launch, whose epilogue does it all; up to 64
-    rows need ``sums`` (float32 [>= rows, N]), where silu(g) * u lies between two launches.  The bits are the same either way."""
+    rows need ``sums`` (float32 [>= rows, N]), where silu(g) * u lies between two launches.  The bits are the same either way.
+    What comes out shares no memory with what goes in."""
     device = _device_of(x, "gemm_fp8_swiglu: x")
     xp, ldx, sp, lds, blocks = _codes_arg(x, x_scales, rows, None, device, "gemm_fp8_swiglu")
     wp, wsp, n = _fp8_matrix_arg(w, w_scales, 2, blocks, device, "gemm_fp8_swiglu")

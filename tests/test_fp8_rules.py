@@ -11,7 +11,7 @@ if build._find_current() is None and build._hipcc() is None:
 P = 1 << 20          # a pointer that a refused call never follows
 
 
-def quantize(x=P, ldx=256, codes=P, ldq=256, scales=P, lds=4, rows=4, width=256):
+def quantize(x=P, ldx=256, codes=2 * P, ldq=256, scales=P, lds=4, rows=4, width=256):
     return ops._fn("bw_quantize_fp8")(x, 0, ldx, codes, ldq, scales, lds, rows, width, None)
 
 
@@ -20,10 +20,11 @@ def test_quantization_refuses():
     assert quantize(width=0) == -2 and quantize(ldx=255) == -2 and quantize(ldq=128) == -2 and quantize(lds=3) == -2
     assert quantize(codes=P + 8) == -3 and quantize(ldq=264) == -3
     assert quantize(rows=2 ** 21, lds=2 ** 21) == -2
+    assert quantize(x=P, codes=P) == -2                                               # rows written over while they are read
 
 
-def norm(x=P, y=P, post=None, gate=None, ldg=0, vec=None, stream=P, out=2 * P, kind=0, ldo=256, scales=None, lds=0, rows=4, dim=256):
-    return ops._fn("bw_norm_add_norm")(x, 256, y, 0, 256, post, 0, 1e-6, gate, 0, ldg, 0, vec, 0, 1.0, stream, 256, P, 0, 1e-6, out, kind, ldo, scales, lds,
+def norm(x=P, y=P, post=None, gate=None, ldg=0, vec=None, stream=P, out=2 * P, kind=0, ldo=256, scales=None, lds=0, rows=4, dim=256, ldx=256, ldy=256, ldst=256):
+    return ops._fn("bw_norm_add_norm")(x, ldx, y, 0, ldy, post, 0, 1e-6, gate, 0, ldg, 0, vec, 0, 1.0, stream, ldst, P, 0, 1e-6, out, kind, ldo, scales, lds,
                                        rows, dim, None)
 
 
@@ -33,12 +34,14 @@ def test_norm_refuses():
     assert norm(out=P) == -2                                                          # both results in one place
     assert norm(kind=2) == -2 and norm(kind=2, scales=P, lds=3) == -2                 # codes without scales, or with too few
     assert norm(kind=2, scales=P, lds=4, out=2 * P + 4) == -3 and norm(kind=2, scales=P, lds=4, ldo=260) == -3
+    assert norm(ldx=255) == -2 and norm(ldy=255) == -2 and norm(ldst=255) == -2 and norm(ldo=255) == -2 and norm(gate=P, ldg=255) == -2
+    assert norm(dim=(1 << 30) + 1) == -2                                              # (an index of eights would pass 32 bits)
     for given in ("post", "gate", "vec"):
         assert norm(y=None, **{given: P}) == -2                                       # nothing to norm, gate or scale
 
 
-def product(x=P, ldx=256, ldxs=4, w=P, residual=None, ldr=64, ldo=64, bf16=0, rows=4, n=64, k=256):
-    return ops._fn("bw_gemm_fp8")(x, ldx, P, ldxs, w, P, residual, ldr, P, ldo, bf16, rows, n, k, None)
+def product(x=P, ldx=256, ldxs=4, w=P, residual=None, ldr=64, ldo=64, bf16=0, rows=4, n=64, k=256, out=2 * P):
+    return ops._fn("bw_gemm_fp8")(x, ldx, P, ldxs, w, P, residual, ldr, out, ldo, bf16, rows, n, k, None)
 
 
 def test_products_refuse():
@@ -47,16 +50,18 @@ def test_products_refuse():
     assert product(ldo=63) == -2 and product(residual=P, ldr=63) == -2 and product(residual=P, bf16=1) == -2
     assert product(x=P + 1) == -3 and product(w=P + 4) == -3 and product(ldx=264) == -3
     assert product(ldx=1 << 24) == -2
+    assert product(out=P) == -2                                                       # (x itself)
 
 
-def gated(x=P, ldx=256, ldxs=4, sums=P, ldsums=64, codes=P, ldq=128, lds=4, rows=4, n=64, k=256):
-    return ops._fn("bw_gemm_fp8_swiglu")(x, ldx, P, ldxs, P, P, sums, ldsums, codes, ldq, P, lds, rows, n, k, None)
+def gated(x=P, ldx=256, ldxs=4, sums=P, ldsums=64, codes=2 * P, ldq=128, lds=4, rows=4, n=64, k=256, scales=3 * P):
+    return ops._fn("bw_gemm_fp8_swiglu")(x, ldx, P, ldxs, P, P, sums, ldsums, codes, ldq, scales, lds, rows, n, k, None)
 
 
 def test_gated_products_refuse():
     assert gated(rows=0) == 0
     assert gated(sums=None) == -2 and gated(ldsums=63) == -2 and gated(ldq=112) == -2 and gated(lds=3) == -2 and gated(k=100) == -2
     assert gated(codes=P + 8) == -3 and gated(ldq=136) == -3
+    assert gated(codes=P) == -2 and gated(scales=P) == -2                             # (x itself, its scales)
 
 
 def test_wrappers_refuse_tensors_off_the_gpu():

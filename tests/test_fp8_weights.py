@@ -93,7 +93,7 @@ def test_random_models_in_8_bits(tmp_path):
 def test_a_config_of_other_blocks_is_refused():
     cfg = dict(tiny.CONFIGS["A"][0])
     LlamaConfig.from_dict(dict(cfg, quantization_config={"quant_method": "fp8", "fmt": "e4m3", "weight_block_size": [128, 128]}))
-    for other in ({"quant_method": "gptq"}, {"quant_method": "fp8", "weight_block_size": [64, 64]}, {"quant_method": "fp8"},
+    for other in ("fp8", {"quant_method": "gptq"}, {"quant_method": "fp8", "weight_block_size": [64, 64]}, {"quant_method": "fp8"},
                   {"quant_method": "fp8", "fmt": "e5m2", "weight_block_size": [128, 128]},
                   {"quant_method": "fp8", "weight_block_size": [128, 128], "activation_scheme": "static"}):
         with pytest.raises(ConfigError, match="quantization_config"):
