@@ -492,13 +492,12 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
       uint32_t mx = 0u;
 #pragma unroll
       for (int v = 0; v < T::WX; ++v) mx = max_bits(mx, most[v * BM + row]);
-      const float scale = fp8_scale_of(mx);
-      const float inv = 1.0f / scale;
+      const Fp8Scale s = fp8_scale_of(mx);
 #pragma unroll
       for (int j = 0; j < NH; ++j)
         *reinterpret_cast<uint32_t*>(ring + CODES_AT + row * CLD + 16 * (NH * wx + j) + 4 * g) =
-            fp8_codes4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], inv);
-      if (m < a.M && wx == 0 && g == 0) a.out_scales[(size_t)(n0 / BW_FP8_BLOCK) * a.lds + m] = scale;
+            fp8_codes4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], s);
+      if (m < a.M && wx == 0 && g == 0) a.out_scales[(size_t)(n0 / BW_FP8_BLOCK) * a.lds + m] = s.scale;
     }
     __syncthreads();
 #pragma unroll

@@ -2130,9 +2130,9 @@ def _device_of(t: torch.Tensor, what: str) -> int:
 def quantize_fp8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, rows: int) -> None:
     """x[:rows] (bfloat16 or float32, rows a stride apart) as e4m3 codes with a scale for each block of 128 elements of a row:
 
-        scales[b, r] = max(max |x[r, block b]|, 448 * 2^-126) / 448,  codes[r, k] = e4m3(x[r, k] * (1 / scales[b, r]))
+        m = max(max |x[r, block b]|, 448 * 2^-126),  scales[b, r] = m / 448,  codes[r, k] = e4m3(448 * x[r, k] / m)
 
-    all in 32 bits, the codes rounded to nearest even.  ``codes`` [>= rows, fp8_width(K)] gets zeros behind the rows' end;
+    with quotients rounded to 32 bits once, the codes to nearest even.  ``codes`` [>= rows, fp8_width(K)] gets zeros behind the rows' end;
     ``scales`` [fp8_width(K) / 128, >= rows].  A block that holds an infinity or NaN stands for NaN throughout.
     ``codes`` is memory of its own."""
     if x.dtype not in (_BF16, _F32) or x.dim() != 2:

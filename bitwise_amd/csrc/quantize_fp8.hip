@@ -20,11 +20,10 @@ __global__ __launch_bounds__(256) void quantize_fp8_kernel(const void* __restric
   const Raw8 raw = load_raw8<VEC>(x, x_is_bf16, (size_t)(in ? row : 0) * ldx, e, width);
   float v[8];
   raw8_floats<VEC>(raw, x_is_bf16, v);
-  const float scale = fp8_scale_of(row16_max_bits(largest8(v)));
-  const float inv = 1.0f / scale;
+  const Fp8Scale s = fp8_scale_of(row16_max_bits(largest8(v)));
   if (!in) return;
-  *reinterpret_cast<u32x2*>(codes + (size_t)row * ldq + e) = (u32x2){fp8_codes4(v[0], v[1], v[2], v[3], inv), fp8_codes4(v[4], v[5], v[6], v[7], inv)};
-  if (l == 0) scales[(size_t)block * lds + row] = scale;
+  *reinterpret_cast<u32x2*>(codes + (size_t)row * ldq + e) = (u32x2){fp8_codes4(v[0], v[1], v[2], v[3], s), fp8_codes4(v[4], v[5], v[6], v[7], s)};
+  if (l == 0) scales[(size_t)block * lds + row] = s.scale;
 }
 
 // ------------------------------------------------------------------------------ the norms around a sublayer
@@ -86,11 +85,10 @@ __device__ __forceinline__ void store_normed(const NormAddNormArgs& a, size_t ro
 #pragma unroll
   for (int i = 0; i < 8; ++i) h[i] = (x[i] * inv) * w[i];
   if (a.out_kind == OUT_FP8) {
-    const float scale = fp8_scale_of(row16_max_bits(largest8(h)));
-    const float q = 1.0f / scale;
+    const Fp8Scale s = fp8_scale_of(row16_max_bits(largest8(h)));
     if (e < whole) {
-      *reinterpret_cast<u32x2*>((uint8_t*)a.out + row * a.ldo + e) = (u32x2){fp8_codes4(h[0], h[1], h[2], h[3], q), fp8_codes4(h[4], h[5], h[6], h[7], q)};
-      if ((e & (BW_FP8_BLOCK - 1)) == 0) a.scales[(size_t)(e / BW_FP8_BLOCK) * a.lds + row] = scale;
+      *reinterpret_cast<u32x2*>((uint8_t*)a.out + row * a.ldo + e) = (u32x2){fp8_codes4(h[0], h[1], h[2], h[3], s), fp8_codes4(h[4], h[5], h[6], h[7], s)};
+      if ((e & (BW_FP8_BLOCK - 1)) == 0) a.scales[(size_t)(e / BW_FP8_BLOCK) * a.lds + row] = s.scale;
     }
   } else if (a.out_kind == OUT_BF16) {
     bf16_t* to = (bf16_t*)a.out + row * a.ldo + e;

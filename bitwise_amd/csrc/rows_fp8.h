@@ -2,11 +2,13 @@
 // (quantize_fp8.hip, gemm_fp8.hip).  A row of K elements has whole blocks of codes, zeros behind its end; the scale of block b
 // of row r lies at scales[b * ld + r], block by block, so that a product's 16 rows find a block's scales side by side.
 //
-//   scale = max(max |x|, 448 * 2^-126) / 448,  code = e4m3(x * (1 / scale)), rounded to nearest even
+//   m = max(max |x|, 448 * 2^-126),  scale = m / 448,  code = e4m3(448 x / m), rounded to nearest even
 //
-// with the division and the reciprocal correctly rounded: a block of zeros has the scale 2^-126, no quotient overflows (the
-// largest magnitude gives 448 within two units in the last place, and 448 is what all up to 464 round to), and every
-// route to a row gives the same bits.  A block with an infinity or NaN has an infinite or NaN scale: everything in it stands for NaN.
+// The quotient is the 32-bit number nearest to 448 x / m: the factor 448 / m stays in two parts (with its rounded value alone, or with
+// the rounded scale, elements that lie halfway between two codes go to either: of rows of bfloat16 numbers, which have many of those, 1 in
+// 2,000, and their values were 2e-3 of the rows' norm off the definition's).  A block of zeros has the scale 2^-126, no quotient
+// overflows, and every route to a row gives the same bits.  A block with an infinity or NaN has an infinite or NaN scale and
+// NaN for codes: everything in it stands for NaN.
 #pragma once
 
 #include "common.h"
@@ -24,14 +26,22 @@ __device__ __forceinline__ uint32_t row16_max_bits(uint32_t v) {
   return max_bits(v, __float_as_uint(lane_xor<1>(__uint_as_float(v))));
 }
 
-__device__ __forceinline__ float fp8_scale_of(uint32_t amax_bits) {
-  return __uint_as_float(max_bits(amax_bits, __float_as_uint(448.0f * 0x1p-126f))) / 448.0f;
+// A block's scale, and 448 / m = hi + lo (off by 2^-47 of it).
+struct Fp8Scale {
+  float scale, hi, lo;
+};
+
+__device__ __forceinline__ Fp8Scale fp8_scale_of(uint32_t amax_bits) {
+  const float m = __uint_as_float(max_bits(amax_bits, __float_as_uint(448.0f * 0x1p-126f)));
+  const float hi = 448.0f / m;
+  return {m / 448.0f, hi, (fmaf(-hi, m, 448.0f) * (1.0f / 448.0f)) * hi};
 }
 
-// Four codes of four values times the scale's reciprocal.
-__device__ __forceinline__ uint32_t fp8_codes4(float a, float b, float c, float d, float inv) {
-  int v = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, v, true);
+// Four codes of four values.
+__device__ __forceinline__ uint32_t fp8_codes4(float a, float b, float c, float d, const Fp8Scale& s) {
+  auto quotient = [&](float x) { return fmaf(x, s.hi, x * s.lo); };
+  int v = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(a), quotient(b), 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(quotient(c), quotient(d), v, true);
 }
 
 // Eight consecutive elements as they come from memory: 16 bytes of bfloat16 or 32 of floats.  The load is a step of its own, so

@@ -23,13 +23,13 @@ def codes_like(rows, width, gpu, more=0, fill=0x2a):
 
 
 def quantized(x):
-    """The definition, each step one 32-bit operation, on the CPU: codes [rows, whole blocks] and scales [blocks, rows]."""
+    """The definition on the CPU, scales and quotients rounded to 32 bits once: codes [rows, whole blocks] and scales [blocks, rows]."""
     x = x.float()
     kp = ops.fp8_width(x.shape[1])
     b = torch.nn.functional.pad(x, (0, kp - x.shape[1])).view(x.shape[0], kp // 128, 128)
     amax = b.abs().amax(dim=2)
-    scale = torch.where(amax < 448.0 * TINY, torch.tensor(448.0 * TINY), amax) / 448.0
-    return (b * (1.0 / scale)[:, :, None]).view(x.shape[0], kp).to(F8), scale.t().contiguous()
+    most = torch.where(amax < 448.0 * TINY, torch.tensor(448.0 * TINY), amax)
+    return (448.0 * b.double() / most.double()[:, :, None]).float().view(x.shape[0], kp).to(F8), (most / 448.0).t().contiguous()
 
 
 def values(codes, scales):

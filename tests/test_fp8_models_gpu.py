@@ -22,8 +22,8 @@ def quantized_rows(x):
     x32 = x.to(torch.float32)
     kb = -(-x32.shape[1] // 128)
     b = torch.nn.functional.pad(x32, (0, kb * 128 - x32.shape[1])).view(x32.shape[0], kb, 128)
-    scale = b.abs().amax(2, keepdim=True).clamp_min(448.0 * 2.0 ** -126) / 448.0
-    return ((b * (1.0 / scale)).to(torch.float8_e4m3fn).double() * scale.double()).view(x32.shape[0], -1)[:, :x32.shape[1]]
+    most = b.abs().amax(2, keepdim=True).clamp_min(448.0 * 2.0 ** -126)
+    return ((448.0 * b.double() / most.double()).float().to(torch.float8_e4m3fn).double() * (most / 448.0).double()).view(x32.shape[0], -1)[:, :x32.shape[1]]
 
 
 def plain_8bit(config, w, tokens):
