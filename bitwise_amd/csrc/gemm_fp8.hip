@@ -13,6 +13,8 @@
 // of a multiply-add, runs beside the matrix instructions.
 //
 // Rows of codes and of the matrix have whole blocks (zeros behind the inner size).
+#include <type_traits>
+
 #include "rows_fp8.h"
 #include "api.h"
 
@@ -121,47 +123,62 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
     voff_x[i] = 16 * i + r < rows ? (16 * i + r) * a.ldx + 16 * g : OUTSIDE;
     row_m[i] = m0 + min(16 * i + r, rows - 1);
   }
-  const float* ws_row[NB];
+  __amdgpu_buffer_rsrc_t rs_ws[NB];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) ws_row[b] = a.ws + ((size_t)(n0 / BW_FP8_BLOCK) + (size_t)b * ((a.N + BW_FP8_BLOCK - 1) / BW_FP8_BLOCK)) * KB;
+  for (int b = 0; b < NB; ++b)
+    rs_ws[b] = rows_of(a.ws + ((size_t)(n0 / BW_FP8_BLOCK) + (size_t)b * ((a.N + BW_FP8_BLOCK - 1) / BW_FP8_BLOCK)) * KB, (size_t)KB * 4);
 
   u32x4 wq[D][NS][2], xq[D][WM][2];
   float sx[D][WM], sw[D][NB];
+  // (A wave whose turn lies behind the last block asks memory for nothing: 8 x 28672 x 4224, a block past whole passes, 31.5 -> 29.3 us.
+  // All are vector loads, in one order everywhere and in the last pass not at all: they return in order, so that a wait for a block's
+  // codes leaves the loads behind them in flight, where loads behind a branch made it a wait for everything.  Factors last were slower,
+  // 64 x 6144 x 4096 18.3 for 16.6.)
   auto issue = [&](int d, int pass) {
-    const int blk = min((pass * D + d) * NW + wave, KB - 1);     // (past the end: the last block again, whose sums nobody takes)
+    const int blk = (pass * D + d) * NW + wave, at_k = blk < KB ? blk * BW_FP8_BLOCK : OUTSIDE;
+#pragma unroll
+    for (int i = 0; i < WM; ++i) sx[d][i] = a.xs[(size_t)min(blk, KB - 1) * a.ldxs + row_m[i]];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) sw[d][b] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs_ws[b], 0, blk * 4, 0));
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const int at = voff_w + c * CW * a.K;                    // (a strip past the matrix lies outside the descriptor)
-        wq[d][c * NB + b][0] = __builtin_amdgcn_raw_buffer_load_b128(rs_w[b], at, blk * BW_FP8_BLOCK, 0);
-        wq[d][c * NB + b][1] = __builtin_amdgcn_raw_buffer_load_b128(rs_w[b], at + 64, blk * BW_FP8_BLOCK, 0);
+        wq[d][c * NB + b][0] = __builtin_amdgcn_raw_buffer_load_b128(rs_w[b], at, at_k, 0);
+        wq[d][c * NB + b][1] = __builtin_amdgcn_raw_buffer_load_b128(rs_w[b], at + 64, at_k, 0);
       }
 #pragma unroll
     for (int i = 0; i < WM; ++i) {
-      xq[d][i][0] = __builtin_amdgcn_raw_buffer_load_b128(rs_x, voff_x[i], blk * BW_FP8_BLOCK, 0);
-      xq[d][i][1] = __builtin_amdgcn_raw_buffer_load_b128(rs_x, voff_x[i] + 64, blk * BW_FP8_BLOCK, 0);
+      xq[d][i][0] = __builtin_amdgcn_raw_buffer_load_b128(rs_x, voff_x[i], at_k, 0);
+      xq[d][i][1] = __builtin_amdgcn_raw_buffer_load_b128(rs_x, voff_x[i] + 64, at_k, 0);
     }
-#pragma unroll
-    for (int i = 0; i < WM; ++i) sx[d][i] = a.xs[(size_t)blk * a.ldxs + row_m[i]];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) sw[d][b] = ws_row[b][blk];
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // the outputs that this thread owns
+  auto owned = [&](int o, int& m, int& n) {
+    const int e = (int)threadIdx.x + o * 64 * NW;
+    m = m0 + 16 * (e / PS % WM) + ((e >> 2) & 15);
+    n = n0 + CW * (e / (PS * WM)) + 4 * ((e % PS) >> 6) + (e & 3);
+    return e < OWNED && m < a.M && n < a.N;
   };
   const int passes = (KB + C - 1) / C;
 #pragma unroll
   for (int d = 0; d < D; ++d) issue(d, 0);
-  __builtin_amdgcn_sched_barrier(0);
-  float acc[NB][OWN];
+  float acc[NB][OWN], old[OWN];                                  // (old: what the sums are added to, asked for early)
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
+  for (int o = 0; o < OWN; ++o) {
 #pragma unroll
-    for (int o = 0; o < OWN; ++o) acc[b][o] = 0.0f;
-  for (int pass = 0; pass < passes; ++pass) {
-    if (pass > 0) lds_barrier();                                 // (the sums of the pass before have been walked)
+    for (int b = 0; b < NB; ++b) acc[b][o] = 0.0f;
+    int m, n;
+    if (EPI == STORE_F32 && a.residual != nullptr && owned(o, m, n)) old[o] = a.residual[(size_t)m * a.ldr + n];
+  }
+  auto run = [&](int pass, auto is_last) {
+    constexpr bool LAST = decltype(is_last)::value;
 #pragma unroll
     for (int d = 0; d < D; ++d) {
       const int at = d * NW + wave;
-      if (pass * C + at < KB) {                                  // (scalar)
+      if (!LAST || pass * C + at < KB) {                         // (scalar)
         Frag fw[NS];
 #pragma unroll
         for (int k = 0; k < NS; ++k) fw[k] = frag_of(wq[d][k][0], wq[d][k][1]);
@@ -179,11 +196,10 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
           }
         }
       }
-      if (pass + 1 < passes) issue(d, pass + 1);
-      __builtin_amdgcn_sched_barrier(0);
+      if (!LAST) issue(d, pass + 1);
     }
     lds_barrier();
-    const int here = min(C, KB - pass * C);
+    const int here = LAST ? KB - pass * C : C;
 #pragma unroll
     for (int o = 0; o < OWN; ++o) {
       const int e = (int)threadIdx.x + o * 64 * NW;
@@ -193,7 +209,7 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
 #pragma unroll
           for (int b = 0; b < NB; ++b) acc[b][o] = fmaf(factor[(v * NB + b) * (WM * 16) + m], part[(v * NB + b) * OWNED + e], acc[b][o]);
         };
-        if (here == C) {
+        if (!LAST || here == C) {
 #pragma unroll 16
           for (int v = 0; v < C; ++v) walk(v);
         } else {
@@ -202,12 +218,18 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
         }
       }
     }
+  };
+  for (int pass = 0; pass < passes - 1; ++pass) {
+    run(pass, std::false_type{});
+    lds_barrier();                                               // (the pass's sums have been walked)
   }
+  run(passes - 1, std::true_type{});
 #pragma unroll
   for (int o = 0; o < OWN; ++o) {
-    const int e = (int)threadIdx.x + o * 64 * NW;
-    const int m = m0 + 16 * (e / PS % WM) + ((e >> 2) & 15), n = n0 + CW * (e / (PS * WM)) + 4 * ((e % PS) >> 6) + (e & 3);
-    if (e < OWNED && m < a.M && n < a.N) store_one<EPI>(a, m, n, acc[0][o], acc[NB - 1][o]);
+    int m, n;
+    if (!owned(o, m, n)) continue;
+    if (EPI == STORE_F32) ((float*)a.out)[(size_t)m * a.ldo + n] = a.residual != nullptr ? old[o] + acc[0][o] : acc[0][o];
+    else store_one<EPI>(a, m, n, acc[0][o], acc[NB - 1][o]);
   }
 }
 
