@@ -74,6 +74,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* base, size
   return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
 }
 
+// 16 bytes a lane from memory to LDS, lane l's to ``to`` + 16 l.
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rs, unsigned char* to, int voff, int soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)to, 16, voff, soff, 0, 0);
+}
+
 constexpr int OUTSIDE = 0x7fff0000;           // an offset behind every descriptor's end: reads as zeros, asks memory for nothing
 
 __device__ __forceinline__ void lds_barrier() {
@@ -97,61 +102,100 @@ __device__ __forceinline__ void store_one(const Fp8Args& a, int m, int n, float 
 
 // ------------------------------------------------------------------------------ few rows
 
+// Offsets behind the descriptors of up to 64 rows (of at most 2^23 bytes), whose sums stay below 2^31.
+constexpr int FAR = 0x40000000, BEHIND = 0x30000000;
+
+// How a wave gets its block's rows: straight into registers as the matrix instructions take them, or by way of LDS (a room of its own,
+// 128 bytes a row as in the tiles below), where each load brings eight whole rows; ROOM8: with room for eight rows of x only.
+enum { STRAIGHT = 0, ROOM16 = 1, ROOM8 = 2 };
+
+constexpr int SIXTEEN = 100;                  // the choice of strips for up to 16 rows
+
 // A workgroup of NW waves a block of 16 WM rows of x and NC strips of CW matrix rows (gated: as many gate and up rows).  The blocks of
-// K go round the waves, D to a wave and pass, all asked for before any is waited for; their sums meet in LDS, where the threads that
-// own the outputs walk them in order.  CW = 8 halves a strip (lanes with r >= 8 ask for nothing): twice as many workgroups, for
-// products with too few columns to give every compute unit 16.  More strips a workgroup share x's loads and its conversion.
-// Bound by the matrix's bytes and, at a few us, by what is not overlapped with them: 8 rows of 6144 columns, K = 4096, 7.8 us of
-// which loading alone takes 6 to 6.7, x 0.7 to 1.5, the walk 0.2 to 0.6 (a launch's start and end are 2); 28672 columns 27 us, 4.4 TB/s.
-template <int WM, int NC, int EPI, int NW, int D, int CW>
+// K go round the waves; their sums meet in LDS, where the threads that own the outputs walk them in order.  CW = 8 halves a strip
+// (nothing is asked for for lanes with r >= 8): twice as many workgroups, for products with too few columns to give every compute unit 16.
+// More strips a workgroup share x's loads and its conversion.
+//
+// Bound by the matrix's bytes where it is large (8 x 28672 x 4096 24.9 us, 4.7 TB/s), else by loads, start and end: of 43 x 4096 x 4096
+// straight into registers 10.8 us, 2.7 went with the loads of x, 4.0 with the matrix's, nothing with conversions and walk.  Straight loads
+// have 16 lanes in a row at 16 different lines, which the first cache looks up one by one, some 16 bytes a clock; by way of LDS eight lanes
+// share a line: 8.4 us (64 x 2048 x 8192 13.6 -> 10.0, 8 x 28672 x 4096 27.9 -> 24.9).
+template <int WM, int NC, int EPI, int NW, int CW, int VIA>
 __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
   constexpr int NB = EPI == SWIGLU_F32 ? 2 : 1, NS = NB * NC;                    // (strip c of gate or up b: c * NB + b)
-  constexpr int PS = 16 * CW, OWNED = NC * WM * PS, OWN = (OWNED + 64 * NW - 1) / (64 * NW), C = NW * D;
-  extern __shared__ __attribute__((aligned(16))) float part[];                  // [C][NB][NC][WM][PS], then the factors
-  float* factor = part + C * NB * OWNED;                                        // [C][NB][WM * 16]
+  constexpr int PS = 16 * CW, OWNED = NC * WM * PS, OWN = (OWNED + 64 * NW - 1) / (64 * NW);
+  constexpr int BX = VIA == ROOM8 ? 1 : 2 * WM, BW = CW * NS / 8, ROOM = VIA ? (BX + BW) * 1024 : 0;      // (BX, BW: eights of rows)
+  static_assert(VIA != ROOM8 || WM == 1, "eight rows are one block of x");
+  extern __shared__ __attribute__((aligned(16))) unsigned char room[];          // [NW][ROOM]
+  float* part = reinterpret_cast<float*>(room + NW * ROOM);                     // [NW][NB][NC][WM][PS], then the factors
+  float* factor = part + NW * NB * OWNED;                                       // [NW][NB][WM * 16]
   const int wave = wave_index(), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * (CW * NC), m0 = blockIdx.y * (16 * WM), KB = a.K / BW_FP8_BLOCK;
+  // workgroups with the same strips and other rows are neighbours on one die (every eighth), which reads the strips once
+  const int of_eight = blockIdx.x / (8 * a.m_tiles);
+  const int n0 = (8 * of_eight + (int)(blockIdx.x & 7)) * (CW * NC), m0 = (int)(blockIdx.x / 8 - of_eight * a.m_tiles) * (16 * WM), KB = a.K / BW_FP8_BLOCK;
+  if (n0 >= a.N) return;
   const int rows = min(16 * WM, a.M - m0);
-  __amdgpu_buffer_rsrc_t rs_w[NB];
+  __amdgpu_buffer_rsrc_t rs_w[NB], rs_ws[NB];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) rs_w[b] = rows_of(a.w + ((size_t)b * a.N + n0) * a.K, (size_t)min(CW * NC, a.N - n0) * a.K);
-  const __amdgpu_buffer_rsrc_t rs_x = rows_of(a.x + (size_t)m0 * a.ldx, (size_t)(rows - 1) * a.ldx + a.K);
-  const int voff_w = r < CW ? r * a.K + 16 * g : OUTSIDE;
-  int voff_x[WM], row_m[WM];
-#pragma unroll
-  for (int i = 0; i < WM; ++i) {
-    voff_x[i] = 16 * i + r < rows ? (16 * i + r) * a.ldx + 16 * g : OUTSIDE;
-    row_m[i] = m0 + min(16 * i + r, rows - 1);
-  }
-  __amdgpu_buffer_rsrc_t rs_ws[NB];
-#pragma unroll
-  for (int b = 0; b < NB; ++b)
+  for (int b = 0; b < NB; ++b) {
+    rs_w[b] = rows_of(a.w + ((size_t)b * a.N + n0) * a.K, (size_t)min(CW * NC, a.N - n0) * a.K);
     rs_ws[b] = rows_of(a.ws + ((size_t)(n0 / BW_FP8_BLOCK) + (size_t)b * ((a.N + BW_FP8_BLOCK - 1) / BW_FP8_BLOCK)) * KB, (size_t)KB * 4);
+  }
+  const __amdgpu_buffer_rsrc_t rs_x = rows_of(a.x + (size_t)m0 * a.ldx, (size_t)(rows - 1) * a.ldx + a.K);
+  int row_m[WM];
+#pragma unroll
+  for (int i = 0; i < WM; ++i) row_m[i] = m0 + min(16 * i + r, rows - 1);
+  // STRAIGHT: a lane's rows.  Otherwise: a load's row and slot of a lane (``via``), and where it reads its operands (of 16 rows, of 8).
+  int voff_w = 0, voff_x[WM], via_x[2], via_w[2], from16[2], from8[2];
+  unsigned char* const mine = room + wave * ROOM;
+  if constexpr (VIA == STRAIGHT) {
+    voff_w = r < CW ? r * a.K + 16 * g : FAR;
+#pragma unroll
+    for (int i = 0; i < WM; ++i) voff_x[i] = 16 * i + r < rows ? (16 * i + r) * a.ldx + 16 * g : FAR;
+  } else {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int lrow = lane >> 3, chunk = 16 * ((lane & 7) ^ (4 * t + (lrow >> 1)));
+      via_x[t] = lrow * a.ldx + chunk;
+      via_w[t] = lrow * a.K + chunk;
+      from16[t] = r * 128 + (((4 * t + g) ^ (r >> 1)) * 16);
+      from8[t] = (r & 7) * 128 + (((4 * t + g) ^ ((r & 7) >> 1)) * 16);
+    }
+  }
 
-  u32x4 wq[D][NS][2], xq[D][WM][2];
-  float sx[D][WM], sw[D][NB];
+  u32x4 wq[NS][2], xq[WM][2];
+  float sx[WM], sw[NB];
   // (A wave whose turn lies behind the last block asks memory for nothing: 8 x 28672 x 4224, a block past whole passes, 31.5 -> 29.3 us.
-  // All are vector loads, in one order everywhere and in the last pass not at all: they return in order, so that a wait for a block's
-  // codes leaves the loads behind them in flight, where loads behind a branch made it a wait for everything.  Factors last were slower,
-  // 64 x 6144 x 4096 18.3 for 16.6.)
-  auto issue = [&](int d, int pass) {
-    const int blk = (pass * D + d) * NW + wave, at_k = blk < KB ? blk * BW_FP8_BLOCK : OUTSIDE;
+  // All are vector loads, in one order everywhere and in the last pass not at all, so that what is waited for is never more than
+  // needed.  Factors last were slower, 64 x 6144 x 4096 18.3 for 16.6.)
+  auto issue = [&](int pass) {
+    const int blk = pass * NW + wave, at_k = blk < KB ? blk * BW_FP8_BLOCK : BEHIND;
 #pragma unroll
-    for (int i = 0; i < WM; ++i) sx[d][i] = a.xs[(size_t)min(blk, KB - 1) * a.ldxs + row_m[i]];
+    for (int i = 0; i < WM; ++i) sx[i] = a.xs[(size_t)min(blk, KB - 1) * a.ldxs + row_m[i]];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) sw[d][b] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs_ws[b], 0, blk * 4, 0));
+    for (int b = 0; b < NB; ++b) sw[b] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs_ws[b], 0, blk * 4, 0));
+    if constexpr (VIA == STRAIGHT) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int at = voff_w + c * CW * a.K;                    // (a strip past the matrix lies outside the descriptor)
-        wq[d][c * NB + b][0] = __builtin_amdgcn_raw_buffer_load_b128(rs_w[b], at, at_k, 0);
-        wq[d][c * NB + b][1] = __builtin_amdgcn_raw_buffer_load_b128(rs_w[b], at + 64, at_k, 0);
+        for (int b = 0; b < NB; ++b) {
+          const int at = voff_w + c * CW * a.K;                  // (a strip past the matrix lies outside the descriptor)
+          wq[c * NB + b][0] = __builtin_amdgcn_raw_buffer_load_b128(rs_w[b], at, at_k, 0);
+          wq[c * NB + b][1] = __builtin_amdgcn_raw_buffer_load_b128(rs_w[b], at + 64, at_k, 0);
+        }
+#pragma unroll
+      for (int i = 0; i < WM; ++i) {
+        xq[i][0] = __builtin_amdgcn_raw_buffer_load_b128(rs_x, voff_x[i], at_k, 0);
+        xq[i][1] = __builtin_amdgcn_raw_buffer_load_b128(rs_x, voff_x[i] + 64, at_k, 0);
       }
+    } else {
+      // (rows past the matrices lie outside the descriptors: zeros)
 #pragma unroll
-    for (int i = 0; i < WM; ++i) {
-      xq[d][i][0] = __builtin_amdgcn_raw_buffer_load_b128(rs_x, voff_x[i], at_k, 0);
-      xq[d][i][1] = __builtin_amdgcn_raw_buffer_load_b128(rs_x, voff_x[i] + 64, at_k, 0);
+      for (int t = 0; t < BX; ++t) load_to_lds(rs_x, mine + t * 1024, via_x[t & 1], at_k + 8 * t * a.ldx);
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int t = 0; t < BW / NB; ++t) load_to_lds(rs_w[b], mine + (BX + b * (BW / NB) + t) * 1024, via_w[CW == 16 ? t & 1 : 0], at_k + 8 * t * a.K);
     }
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -162,9 +206,8 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
     n = n0 + CW * (e / (PS * WM)) + 4 * ((e % PS) >> 6) + (e & 3);
     return e < OWNED && m < a.M && n < a.N;
   };
-  const int passes = (KB + C - 1) / C;
-#pragma unroll
-  for (int d = 0; d < D; ++d) issue(d, 0);
+  const int passes = (KB + NW - 1) / NW;
+  issue(0);
   float acc[NB][OWN], old[OWN];                                  // (old: what the sums are added to, asked for early)
 #pragma unroll
   for (int o = 0; o < OWN; ++o) {
@@ -175,31 +218,51 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
   }
   auto run = [&](int pass, auto is_last) {
     constexpr bool LAST = decltype(is_last)::value;
+    if (!LAST || pass * NW + wave < KB) {                        // (scalar)
+      if constexpr (VIA != STRAIGHT) {
+        __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+        asm volatile("" ::: "memory");
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
-      const int at = d * NW + wave;
-      if (!LAST || pass * C + at < KB) {                         // (scalar)
-        Frag fw[NS];
+        for (int t = 0; t < 2; ++t) {
 #pragma unroll
-        for (int k = 0; k < NS; ++k) fw[k] = frag_of(wq[d][k][0], wq[d][k][1]);
+          for (int i = 0; i < WM; ++i) xq[i][t] = *reinterpret_cast<const u32x4*>(mine + 2048 * i + (VIA == ROOM8 ? from8[t] : from16[t]));
 #pragma unroll
-        for (int i = 0; i < WM; ++i) {
-          const Frag fx = frag_of(xq[d][i][0], xq[d][i][1]);
+          for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int b = 0; b < NB; ++b) {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-              const f32x4 sums = block_sums(fw[c * NB + b], fx);
-              if (CW == 16 || lane < 32) *reinterpret_cast<f32x4*>(part + (((at * NB + b) * NC + c) * WM + i) * PS + 4 * lane) = sums;
-            }
-            if (g == 0) factor[(at * NB + b) * (WM * 16) + 16 * i + r] = sx[d][i] * sw[d][b];
-          }
+            for (int b = 0; b < NB; ++b)
+              wq[c * NB + b][t] = *reinterpret_cast<const u32x4*>(mine + (BX + (b * NC + c) * (CW / 8)) * 1024 + (CW == 16 ? from16[t] : from8[t]));
         }
       }
-      if (!LAST) issue(d, pass + 1);
+      float both[WM][NB];
+#pragma unroll
+      for (int i = 0; i < WM; ++i)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) both[i][b] = sx[i] * sw[b];
+      if constexpr (VIA != STRAIGHT && !LAST) {
+        __builtin_amdgcn_s_waitcnt(0xc07f);                      // (the block has left its room)
+        asm volatile("" ::: "memory");
+        issue(pass + 1);
+      }
+      Frag fw[NS];
+#pragma unroll
+      for (int k = 0; k < NS; ++k) fw[k] = frag_of(wq[k][0], wq[k][1]);
+#pragma unroll
+      for (int i = 0; i < WM; ++i) {
+        const Frag fx = frag_of(xq[i][0], xq[i][1]);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const f32x4 sums = block_sums(fw[c * NB + b], fx);
+            if (CW == 16 || lane < 32) *reinterpret_cast<f32x4*>(part + (((wave * NB + b) * NC + c) * WM + i) * PS + 4 * lane) = sums;
+          }
+          if (g == 0) factor[(wave * NB + b) * (WM * 16) + 16 * i + r] = both[i][b];
+        }
+      }
     }
+    if (!LAST && VIA == STRAIGHT) issue(pass + 1);
     lds_barrier();
-    const int here = LAST ? KB - pass * C : C;
+    const int here = LAST ? KB - pass * NW : NW;
 #pragma unroll
     for (int o = 0; o < OWN; ++o) {
       const int e = (int)threadIdx.x + o * 64 * NW;
@@ -209,9 +272,9 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
 #pragma unroll
           for (int b = 0; b < NB; ++b) acc[b][o] = fmaf(factor[(v * NB + b) * (WM * 16) + m], part[(v * NB + b) * OWNED + e], acc[b][o]);
         };
-        if (!LAST || here == C) {
-#pragma unroll 16
-          for (int v = 0; v < C; ++v) walk(v);
+        if (!LAST || here == NW) {
+#pragma unroll
+          for (int v = 0; v < NW; ++v) walk(v);
         } else {
 #pragma unroll 4
           for (int v = 0; v < here; ++v) walk(v);
@@ -574,46 +637,52 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 
 // ------------------------------------------------------------------------------ which kernel
 
-template <int WM, int NC, int EPI, int NW, int D, int CW>
-int launch_few(const Fp8Args& a, hipStream_t s) {
-  constexpr int NB = EPI == SWIGLU_F32 ? 2 : 1, LDS = NW * D * NB * WM * 16 * (CW * NC + 1) * 4;
+template <int WM, int NC, int EPI, int NW, int CW, int VIA>
+int launch_few(Fp8Args a, hipStream_t s) {
+  constexpr int NB = EPI == SWIGLU_F32 ? 2 : 1, LDS = NW * (NB * WM * 16 * (CW * NC + 1) * 4 + (VIA ? (VIA == ROOM8 ? 8 : 16 * WM) + CW * NC * NB : 0) * 128);
   static_assert(LDS <= 160 * 1024 && 128 % (CW * NC) == 0, "a pass's sums fit LDS, a workgroup's columns one block's scale");
-  hipLaunchKernelGGL((gemm_fp8_few_kernel<WM, NC, EPI, NW, D, CW>), dim3((a.N + CW * NC - 1) / (CW * NC), (a.M + 16 * WM - 1) / (16 * WM)), dim3(64 * NW), LDS, s,
-                     a);
+  a.m_tiles = (a.M + 16 * WM - 1) / (16 * WM);
+  a.n_tiles = (a.N + CW * NC - 1) / (CW * NC);
+  hipLaunchKernelGGL((gemm_fp8_few_kernel<WM, NC, EPI, NW, CW, VIA>), dim3((unsigned)((a.n_tiles + 7) / 8 * 8 * a.m_tiles)), dim3(64 * NW), LDS, s, a);
   return BW_LAUNCH_CHECK();
 }
 
 // Up to 16 rows: strips of 16 columns for the 256 compute units, K's blocks over the waves of one.  Eight waves a strip where there are
-// strips for more than one workgroup a unit (8 rows of 28672 columns, K = 4096: 27.0 us, with 16 waves 28.2), 16 where there is about
-// one (4096 columns, K = 8192: 10.4, with eight 10.8).  Two strips a workgroup, which halves what x costs, where there are more still
-// and x counts (16 rows of 28672 columns 31.8 -> 29.4 us, 8 of 6144 9.3 -> 8.3, gated 8 x 8192 x 2048 12.4 -> 11.9; but 2 x 16384 x 8192
-// 28.0 -> 31.5).  Up to 2048 columns strips of eight, so that every unit has one: of 2048 columns, K = 2048, 3.4 us for 3.7; K = 8192
-// with all of K asked for at once by 16 waves 8.3 for 9.8, with eight waves 9.0 (K = 2048 so 5.8: most waves have nothing).
-template <int EPI>
+// strips for more than one workgroup a unit (8 rows of 5120 columns, K = 5120: 8.1 us, with 16 waves 10.1), 16 where there is at most
+// one (4 of 4096, K = 14336: 12.7, with eight 14.2).  Up to 2048 columns strips of eight, so that every unit has one: of 2048
+// columns, K = 8192, 6.4 us for 7.2; by eight waves where K has no work for more (K = 1024 2.7 for 2.9).  Up to eight rows leave eight waves room for
+// a fourth workgroup a unit (2 x 16384 x 8192 30.1 -> 27.6 us); with sixteen, one a unit is better (4 x 4096 x 14336 12.7 for 14.5).
+// Two strips a workgroup share x where there is more of it and K is short (16 x 28672 x 2048 15.1 -> 14.2, 16 x 6144 x 4096 9.2 -> 8.5; 16 x 8192 x
+// 8192 16.4 -> 17.2), gated where one workgroup a unit then takes all (3 x 5504 x 2048 9.8 -> 9.0).
+template <int EPI, int VIA>
 int sixteen_rows(const Fp8Args& a, hipStream_t s) {
-  const int KB = a.K / BW_FP8_BLOCK;
-  if (a.N <= 2048) {
-    if constexpr (EPI != SWIGLU_F32) {
-      if (KB > 32 && KB <= 64) return launch_few<1, 1, EPI, 16, 4, 8>(a, s);
-    }
-    return launch_few<1, 1, EPI, 8, 2, 8>(a, s);
-  }
   if constexpr (EPI != SWIGLU_F32) {
-    if (a.N <= 5120) return launch_few<1, 1, EPI, 16, 1, 16>(a, s);
+    if (a.N <= 2048) return a.K <= 8 * BW_FP8_BLOCK ? launch_few<1, 1, EPI, 8, 8, VIA>(a, s) : launch_few<1, 1, EPI, 16, 8, ROOM16>(a, s);
+    if (a.N <= 4096) return launch_few<1, 1, EPI, 16, 16, ROOM16>(a, s);
+    if (VIA == ROOM16 && a.K <= 4096) return launch_few<1, 2, EPI, 8, 16, ROOM16>(a, s);
+  } else {
+    if (a.N > 4096 && a.N <= 8192) return launch_few<1, 2, EPI, 8, 16, VIA>(a, s);
   }
-  if (a.N > 5120 && (EPI == SWIGLU_F32 || a.M > 4)) return launch_few<1, 2, EPI, 8, 1, 16>(a, s);
-  return launch_few<1, 1, EPI, 8, 1, 16>(a, s);
+  return launch_few<1, 1, EPI, 8, 16, VIA>(a, s);
 }
 
 template <int EPI>
 int by_strips(const Fp8Args& a, int shape, hipStream_t s) {
-  switch (shape) {
-    case 0: return launch_few<1, 1, EPI, 8, 1, 16>(a, s);
-    case 1: return launch_few<1, 2, EPI, 8, 1, 16>(a, s);
-    case 2: return launch_few<2, 1, EPI, 8, 1, 16>(a, s);
-    case 3: return launch_few<2, 2, EPI, 8, 1, 16>(a, s);
-    case 4: return launch_few<3, 2, EPI, 8, 1, 16>(a, s);
-    default: return launch_few<4, 2, EPI, 8, 1, 16>(a, s);
+  if (shape == SIXTEEN) return a.M <= 8 ? sixteen_rows<EPI, ROOM8>(a, s) : sixteen_rows<EPI, ROOM16>(a, s);
+  if constexpr (EPI != SWIGLU_F32) {
+    switch (shape) {
+      case 0: return launch_few<1, 1, EPI, 8, 16, ROOM16>(a, s);
+      case 1: return launch_few<1, 2, EPI, 8, 16, ROOM16>(a, s);
+      case 2: return launch_few<2, 1, EPI, 8, 16, ROOM16>(a, s);
+      default: return launch_few<2, 2, EPI, 8, 16, ROOM16>(a, s);
+    }
+  } else {
+    switch (shape) {
+      case 0: return launch_few<2, 1, EPI, 8, 16, STRAIGHT>(a, s);
+      case 1: return launch_few<2, 2, EPI, 8, 16, STRAIGHT>(a, s);
+      case 2: return launch_few<3, 2, EPI, 8, 16, STRAIGHT>(a, s);
+      default: return launch_few<4, 2, EPI, 8, 16, STRAIGHT>(a, s);
+    }
   }
 }
 
@@ -656,11 +725,9 @@ int cheapest(const ShapeCost (&shapes)[SHAPES], int M, int N, int K, double* us)
 }
 
 // Strips: each wave a block of K of its own, which hides what a tile's step waits for; x and the matrix come once a workgroup,
-// though, so many rows and columns are cheaper by tiles (64 x 4096 x 4096 11.2 us by strips, 19.5 by tiles; 40 x 28672 x 4096 49 and 30).
-constexpr ShapeCost STORE_STRIPS[] = {{16, 16, 2, 1.1, 0.115, 1.8, 0.19}, {16, 32, 2, 0.4, 0.173, 0.7, 0.285}, {32, 16, 2, 0.1, 0.20, 0.2, 0.33},
-                                      {32, 32, 2, 0.9, 0.27, 1.5, 0.445}, {48, 32, 1, 2.5, 0.29, 0, 0},        {64, 32, 1, 1.0, 0.44, 0, 0}};
-constexpr ShapeCost GATED_STRIPS[] = {{16, 16, 2, 0.4, 0.20, 0.7, 0.33}, {16, 32, 2, 0.5, 0.28, 0.9, 0.46}, {32, 16, 2, 0.0, 0.285, 0.0, 0.47},
-                                      {32, 32, 1, 0.6, 0.43, 0, 0},      {48, 32, 1, 1.0, 0.55, 0, 0},      {64, 32, 1, 1.0, 0.70, 0, 0}};
+// though, so many rows and columns are cheaper by tiles (64 x 4096 x 4096 9.4 us by strips, 19.6 by tiles; 40 x 28672 x 4096 41 and 31).
+constexpr ShapeCost STORE_STRIPS[] = {{16, 16, 2, 0.1, 0.104, 1.1, 0.154}, {16, 32, 2, 0.2, 0.171, 0.4, 0.306}, {32, 16, 2, 0.2, 0.133, 1.1, 0.225}, {32, 32, 1, 0.8, 0.208, 0, 0}};
+constexpr ShapeCost GATED_STRIPS[] = {{32, 16, 2, 0.0, 0.285, 0.0, 0.47}, {32, 32, 1, 0.6, 0.43, 0, 0}, {48, 32, 1, 1.0, 0.55, 0, 0}, {64, 32, 1, 1.0, 0.70, 0, 0}};
 // Tiles: a step's conversions a matrix instruction fall with the tile.  192 x 256 by eight waves does the most a us, 128 x 128 by four, two
 // workgroups a unit, fills a round sooner, 64 x 128 and 64 x 64 give a few hundred rows of few columns more workgroups.
 constexpr ShapeCost STORE_TILES[] = {{192, 256, 1, 6.5, 2.04, 0, 0}, {128, 128, 2, 5.8, 1.02, 6.5, 1.78}, {64, 128, 2, 2.9, 0.64, 3.1, 1.12}, {64, 64, 2, 2.5, 0.49, 3.2, 0.74}};
@@ -672,7 +739,6 @@ constexpr int FEW_ROWS = 64;                    // rows up to which a gated prod
 
 // What runs: ``strips`` (of the tables above; SIXTEEN: up to 16 rows, the strips made for those), or -1 and ``tiles``, the last ``tail``
 // rows behind the tiles by strips of their own.
-constexpr int SIXTEEN = 100;
 struct Choice {
   int strips, tiles, tail;
 };
@@ -754,7 +820,6 @@ extern "C" int bw_gemm_fp8(const void* x, int ldx, const float* xs, int ldxs, co
               (residual == nullptr || (aligned(residual, 16) && (rows == 1 || ldr % 4 == 0)));
   hipStream_t s = (hipStream_t)stream;
   const Choice c = choose_stored(rows, N, K);
-  if (c.strips == SIXTEEN) return out_is_bf16 ? sixteen_rows<STORE_BF16>(a, s) : sixteen_rows<STORE_F32>(a, s);
   if (c.strips >= 0) return out_is_bf16 ? by_strips<STORE_BF16>(a, c.strips, s) : by_strips<STORE_F32>(a, c.strips, s);
   a.M = rows - c.tail;
   if (const int bad = out_is_bf16 ? stored_by_tiles<STORE_BF16>(a, c.tiles, s) : stored_by_tiles<STORE_F32>(a, c.tiles, s)) return bad;
@@ -788,7 +853,7 @@ extern "C" int bw_gemm_fp8_swiglu(const void* x, int ldx, const float* xs, int l
   if (rows <= FEW_ROWS && (sums == nullptr || (rows > 1 && ldsums < inter))) return -2;
   if (c.strips >= 0) {
     a.out = sums, a.ldo = ldsums;
-    if (const int bad = c.strips == SIXTEEN ? sixteen_rows<SWIGLU_F32>(a, s) : by_strips<SWIGLU_F32>(a, c.strips, s)) return bad;
+    if (const int bad = by_strips<SWIGLU_F32>(a, c.strips, s)) return bad;
     return bw_quantize_fp8(sums, 0, ldsums, codes, ldq, scales, lds, rows, inter, stream);
   }
   a.out = codes, a.ldo = ldq, a.out_scales = scales, a.lds = lds;

@@ -86,12 +86,12 @@ def test_the_gpu_tests_sizes_reach_every_kernel():
     import test_fp8_gpu as sizes
 
     stored = [ops.gemm_fp8_choice(rows, n, ops.fp8_width(k)) for rows, n, k in sizes.STORED]
-    assert {c[0] for c in stored} - {-1} == {*range(6), 100} and {c[1] for c in stored if c[0] < 0 and not c[2]} == set(range(4))
+    assert {c[0] for c in stored} - {-1} == {*range(4), 100} and {c[1] for c in stored if c[0] < 0 and not c[2]} == set(range(4))
     assert len({c[1] for c in stored if c[2]}) >= 3
     long = [ops.gemm_fp8_choice(rows, n, ops.fp8_width(k)) for rows, n, k in sizes.STORED if k > 512]
     assert {c[1] for c in long if c[0] < 0} == set(range(4))
     gated = [ops.gemm_fp8_choice(rows, n, ops.fp8_width(k), gated=True) for rows, n, k in sizes.GATED]
-    assert {c[0] for c in gated} - {-1} == {*range(6), 100} and {c[1] for c in gated if c[0] < 0} == set(range(4))
+    assert {c[0] for c in gated} - {-1} == {*range(4), 100} and {c[1] for c in gated if c[0] < 0} == set(range(4))
     long = [ops.gemm_fp8_choice(rows, n, ops.fp8_width(k), gated=True) for rows, n, k in sizes.GATED if k > 512]
     assert {c[1] for c in long if c[0] < 0} == set(range(4))
     for n, k in ((2048, 2048), (2048, 8192), (4096, 4096), (6144, 4096)):
