@@ -471,7 +471,7 @@ STORED = [(17, 68, 1792), (19, 77, 1536), (17, 70, 128), (18, 4904, 1792), (33, 
           (3348, 261, 128), (1068, 65, 128), (400, 23971, 128), (194, 16868, 128), (1295, 1544, 1920), (960, 4391, 1280),
           (257, 22075, 640), (1001, 4090, 1152), (310, 6005, 1152), (500, 1501, 1152), (60, 6300, 1152),
           (3, 6001, 640), (9, 6001, 640), (16, 3001, 1152), (7, 500, 6144), (16, 500, 2176),
-          (3, 500, 640), (12, 500, 640), (5, 4001, 2176), (60, 1990, 1300), (33, 1990, 700), (9, 4200, 4300)]
+          (3, 500, 640), (12, 500, 640), (5, 4001, 2176), (60, 1990, 1300), (33, 1990, 700), (9, 4200, 4300), (2, 4200, 4300)]
 GATED = [(17, 66, 640), (35, 2069, 384), (17, 67, 128), (17, 4591, 2176), (33, 6263, 384), (49, 6714, 640), (137, 27323, 128), (68, 22010, 128),
          (33, 20016, 128), (68, 65, 128), (132, 22012, 640), (67, 22083, 640), (33, 16470, 640), (200, 5003, 1152), (90, 1501, 1152),
          (3, 6001, 640), (16, 3001, 1152), (7, 500, 6144), (12, 5003, 640), (2, 9001, 640)]
