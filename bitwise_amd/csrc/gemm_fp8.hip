@@ -315,8 +315,8 @@ __device__ __forceinline__ float taken(float v) {
 // What bounds it, of 2048 rows by gated 14336 columns, K = 4096, 404 us (1.19 PFLOP/s; a plain bfloat16 product of the library reaches
 // 1.38): the matrix cores are busy 52 % of the cycles, and for 16 matrix instructions of a wave there are 55 others, of which 27 convert
 // and 18 join chains.  Left out one at a time the conversions are worth 11 %, three quarters of the chains' multiply-adds 8 %, the reads
-// from LDS 9 %, all three together 24 %: then the clock falls with the matrix cores' power (zeros for operands run 8 % faster).  So the
-// tile is as large as a wave's registers allow: a step of 192 x 256 takes 2.04 us, of 128 x 128 for the same work 2.7.
+// from LDS 13 %, the loads 13 %, all together 30 %: no one of them is the bound, and the clock falls with the matrix cores' power
+// (zeros for operands run 8 % faster).  So the tile is as large as a wave's registers allow: a step of 192 x 256 takes 2.04 us, of 128 x 128 for the same work 2.7.
 template <int EPI, int WAVES_, int WY_, int MI_, int NJ_, int ST_>
 struct Fp8Tile {
   static constexpr int WAVES = WAVES_, WY = WY_, WX = WAVES / WY_, MI = MI_, NJ = NJ_, ST = ST_;
