@@ -98,3 +98,15 @@ def test_a_config_of_other_blocks_is_refused():
                   {"quant_method": "fp8", "weight_block_size": [128, 128], "activation_scheme": "static"}):
         with pytest.raises(ConfigError, match="quantization_config"):
             LlamaConfig.from_dict(dict(cfg, quantization_config=other))
+
+
+def test_the_command_line_writes_a_folder_in_8_bits(tmp_path):
+    from bitwise_amd.cli import main
+
+    config = tmp_path / "config.json"
+    config.write_text(json.dumps(tiny.CONFIGS["A"][0]))
+    assert main(["random", "--config", str(config), "--seed", "3", "--weight-dtype", "float8", "--out", str(tmp_path / "m")]) == 0
+    tensors = safetensors_io.read_folder(tmp_path / "m")
+    assert tensors["model.layers.0.self_attn.q_proj.weight"].dtype == torch.float8_e4m3fn
+    assert tensors["model.layers.0.self_attn.q_proj.weight_scale_inv"].dtype == torch.float32
+    assert tensors["model.norm.weight"].dtype == torch.bfloat16
