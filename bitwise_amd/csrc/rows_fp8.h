@@ -101,16 +101,20 @@ __device__ __forceinline__ uint32_t largest8(const float (&v)[8]) {
   return m;
 }
 
-// 1 / (1 + exp(-g)) within two units in the last place: codes are rounded from it, and what is more off moves more of them to
-// a neighbour.  The exponential through the hardware exp2, its argument in two parts; the quotient through the hardware
-// reciprocal and one Newton step.  (Below -88 the argument stays there: silu is off by less than 10^-36.)  NaN gives a number.
+// 1 / (1 + exp(-g)) within two units in the last place (under the normal numbers, within the least number and half of it): codes are
+// rounded from it, and what is more off moves more of them to a neighbour.  The exponential through the hardware exp2, its argument in two
+// parts; the quotient through the hardware reciprocal and one Newton step.  Below -87 the quotient would lie under the normal numbers, which the
+// reciprocal does not give: there 1 + exp(-g) is exp(-g), and exp(g) comes 2^96 too large and is scaled by one product.  Beyond
+// -88 and 112 the argument stays there: the result is 1, or less than half of the least number.  NaN gives a number.
 __device__ __forceinline__ float sigmoid_of_number(float g) {
-  const float x = fminf(-g, 88.0f);
+  const float x = fminf(fmaxf(-g, -88.0f), 112.0f);
   const float hi = x * 0x1.715476p+0f;
   const float lo = fmaf(x, 0x1.715476p+0f, -hi) + x * 0x1.4ae0cp-26f;
-  const float d = fmaf(__builtin_amdgcn_exp2f(hi), fmaf(lo, 0x1.62e43p-1f, 1.0f), 1.0f);
+  const bool small = x > 87.0f;
+  const float e = __builtin_amdgcn_exp2f(small ? 96.0f - hi : hi);
+  const float d = fmaf(e, fmaf(lo, 0x1.62e43p-1f, 1.0f), 1.0f);
   const float r = __builtin_amdgcn_rcpf(d);
-  return fmaf(fmaf(-d, r, 1.0f), r, r);
+  return small ? (e * fmaf(lo, -0x1.62e43p-1f, 1.0f)) * 0x1p-96f : fmaf(fmaf(-d, r, 1.0f), r, r);
 }
 
 __device__ __forceinline__ float sigmoid32(float g) { return g != g ? g : sigmoid_of_number(g); }
