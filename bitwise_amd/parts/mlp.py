@@ -85,7 +85,8 @@ class SwiGLU(FeedForward):
         rt, ws, rows = self.rt, ctx.ws, ctx.rows
         if self.in_codes:
             self._from_codes(ctx, *self.gate_up._quantized(ws, h, rows), residual)
-        elif self.gate_up.mfma:
+            return
+        if self.gate_up.mfma:
             act = ws.buffer("mlp_h", self.inter, torch.bfloat16)
             ops.gemm_bf16(h, self.gate_up.weight, act, rows, ops.EPI_SWIGLU_BF16)   # SwiGLU in the epilogue
         else:
