@@ -6,7 +6,8 @@ number of heads, ``head_dim`` to ``hidden_size // num_attention_heads``,
 ``rope_theta`` to 10000.0, ``rms_norm_eps`` to 1e-6, ``tie_word_embeddings`` to
 False, a list ``eos_token_id`` means its first element, and a truthy
 ``rope_scaling`` is refused (tools/convert.py:59-60), and so is a
-``quantization_config`` of another form than 8-bit codes with a scale for each block of 128 x 128.  ``max_position_embeddings``
+``quantization_config`` of another form than 8-bit codes with a scale for each block of 128 x 128 (a folder whose
+tensors are all stored as plain numbers comes here without one).  ``max_position_embeddings``
 is not read by the reference; here it bounds the rotary table and request lengths.
 """
 

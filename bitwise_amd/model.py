@@ -25,7 +25,7 @@ from .weights import block_scaled, loader
 def model_spec(config: Mapping[str, Any]):
     """The ``ModelSpec`` its architecture makes of a configuration (a config.json dictionary)."""
     arch = registry.architecture_of(config)
-    return arch.spec_from_config(arch.config_from_dict(config))
+    return arch.spec_from_config(arch.config_from_dict(registry.without_quantization(config)))
 
 
 def describe(config: Mapping[str, Any]) -> Dict[str, TensorSpec]:
@@ -40,7 +40,7 @@ def write_random_model(folder: str | Path, config: Mapping[str, Any], seed: int,
     model's tensor order from one generator seeded with ``seed``.  dtype "float8": matrices of the parts that take them so are stored
     in 8 bits with a scale for each block of 128 x 128, the rest in bfloat16."""
     arch = registry.architecture_of(config)
-    typed = arch.config_from_dict(config)
+    typed = arch.config_from_dict(registry.without_quantization(config))
     torch_dtype = {"bfloat16": torch.bfloat16, "float32": torch.float32, "float16": torch.float16, "float8": block_scaled.DTYPE}[dtype]
     return loader.write_model_folder(folder, typed.to_dict(), describe(config), seed, sigma, torch_dtype)
 
@@ -78,7 +78,7 @@ class Model:
                 write_random_model(tmp, config, seed, sigma, weight_dtype)
                 return cls.load(tmp, dtype, device)
         arch = registry.architecture_of(config)
-        typed = arch.config_from_dict(config)
+        typed = arch.config_from_dict(registry.without_quantization(config))
         rt = Runtime(dtype, device)
         assembled = AssembledModel(arch.spec_from_config(typed), rt)
         gen = torch.Generator(device=rt.device)

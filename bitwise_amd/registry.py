@@ -62,17 +62,25 @@ def architecture_of(config: Mapping[str, Any]) -> Architecture:
 
 def read_model_config(folder: str | Path) -> Dict[str, Any]:
     """config.json of a model folder, completed from the shapes in its safetensors headers where the architecture
-    takes sizes from there."""
+    takes sizes from there.  What it says of quantization is left out where every tensor is stored as plain numbers."""
     from .weights import safetensors_io
     raw = read_config(folder)
     arch = architecture_of(raw)
+    if arch.sizes_from_tensors is None and not raw.get("quantization_config"):
+        return raw
+    headers: Dict[str, Any] = {}
+    for shard in sorted(Path(folder).glob("*.safetensors")):
+        headers.update(safetensors_io.read_header(shard)[0])
+    if all(info["dtype"] in safetensors_io.PLAIN for info in headers.values()):
+        raw = without_quantization(raw)
     if arch.sizes_from_tensors is not None:
-        shapes: Dict[str, tuple] = {}
-        for shard in sorted(Path(folder).glob("*.safetensors")):
-            header, _ = safetensors_io.read_header(shard)
-            shapes.update({name: tuple(int(s) for s in info["shape"]) for name, info in header.items()})
-        raw = arch.sizes_from_tensors(raw, shapes)
+        raw = arch.sizes_from_tensors(raw, {name: tuple(int(s) for s in info["shape"]) for name, info in headers.items()})
     return raw
+
+
+def without_quantization(config: Mapping[str, Any]) -> Dict[str, Any]:
+    """A configuration for weights that are not quantized as it may say: another folder's, or those drawn at random."""
+    return {key: v for key, v in config.items() if key != "quantization_config"}
 
 
 def read_config(folder: str | Path) -> Dict[str, Any]:

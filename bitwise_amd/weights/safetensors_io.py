@@ -19,6 +19,7 @@ import torch
 _NP_OF = {"F32": np.float32, "F16": np.float16, "BF16": np.uint16, "F8_E4M3": np.uint8, "I32": np.int32, "I64": np.int64}
 _TORCH_TAG = {torch.float32: "F32", torch.float16: "F16", torch.bfloat16: "BF16", torch.float8_e4m3fn: "F8_E4M3",
               torch.int32: "I32", torch.int64: "I64"}
+PLAIN = ("BF16", "F16", "F32", "F64")          # tensors that stand for themselves
 
 
 class SafetensorsError(ValueError):
