@@ -83,7 +83,8 @@ class LlamaConfig:
                 raise ConfigError(f"{key}=true is not supported by the Llama parts of this engine")
         quantized = d.get("quantization_config")
         if quantized and (not isinstance(quantized, Mapping) or quantized.get("quant_method") != "fp8" or quantized.get("fmt", "e4m3") != "e4m3"
-                          or quantized.get("activation_scheme", "dynamic") != "dynamic" or list(quantized.get("weight_block_size") or []) != [128, 128]):
+                          or quantized.get("activation_scheme", "dynamic") != "dynamic"
+                          or quantized.get("weight_block_size") not in ([128, 128], (128, 128))):
             raise ConfigError("quantization_config: matrices in 8 bits are e4m3 codes with a scale for each block of 128 x 128 (quant_method "
                               f"'fp8', weight_block_size [128, 128], inputs quantized as they come), got {quantized}")
         act = d.get("hidden_act", "silu")

@@ -50,3 +50,9 @@ def test_random_weights_are_stored_as_asked_whatever_the_config_says(tmp_path, q
     assert describe(config) == describe(tiny.CONFIGS["A"][0]) and model_spec(config) == model_spec(tiny.CONFIGS["A"][0])
     folder = write_random_model(tmp_path, config, 3, 0.05)
     assert "quantization_config" not in json.loads((folder / "config.json").read_text())
+
+
+@pytest.mark.parametrize("blocks", [128, "128", None, {}, [128], [128, 128, 128], [[128, 128]]])
+def test_sizes_of_blocks_that_are_no_pair_are_refused(blocks):
+    with pytest.raises(ConfigError, match="quantization_config"):
+        LlamaConfig.from_dict(dict(tiny.CONFIGS["A"][0], quantization_config={"quant_method": "fp8", "weight_block_size": blocks}))
