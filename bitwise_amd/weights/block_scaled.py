@@ -11,6 +11,8 @@ import torch
 BLOCK = 128
 DTYPE = torch.float8_e4m3fn
 SCALE_SUFFIX = "_scale_inv"
+# what a folder's config.json says of such tensors ("quantization_config")
+CONFIG = {"quant_method": "fp8", "fmt": "e4m3", "activation_scheme": "dynamic", "weight_block_size": [BLOCK, BLOCK]}
 
 
 def blocks(n: int) -> int:

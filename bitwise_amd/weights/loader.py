@@ -174,9 +174,12 @@ def random_tensors(specs: Mapping[str, TensorSpec], seed: int, sigma: float = 0.
 
 def write_model_folder(folder: str | Path, config: Mapping[str, object], specs: Mapping[str, TensorSpec],
                        seed: int, sigma: float = 0.02, dtype: torch.dtype = torch.bfloat16) -> Path:
-    """Random-weights mode: ``folder/config.json`` and ``folder/model.safetensors``."""
+    """Random-weights mode: ``folder/config.json`` (which says so if matrices are in 8 bits) and ``folder/model.safetensors``."""
     folder = Path(folder)
     folder.mkdir(parents=True, exist_ok=True)
-    (folder / "config.json").write_text(json.dumps(dict(config), indent=1))
+    said = dict(config)
+    if dtype == block_scaled.DTYPE and any(s.block_scaled for s in specs.values()):
+        said["quantization_config"] = block_scaled.CONFIG
+    (folder / "config.json").write_text(json.dumps(said, indent=1))
     safetensors_io.write_file(folder / "model.safetensors", random_tensors(specs, seed, sigma, dtype))
     return folder

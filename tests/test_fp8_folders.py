@@ -56,3 +56,16 @@ def test_random_weights_are_stored_as_asked_whatever_the_config_says(tmp_path, q
 def test_sizes_of_blocks_that_are_no_pair_are_refused(blocks):
     with pytest.raises(ConfigError, match="quantization_config"):
         LlamaConfig.from_dict(dict(tiny.CONFIGS["A"][0], quantization_config={"quant_method": "fp8", "weight_block_size": blocks}))
+
+
+@pytest.mark.parametrize("name", ["LlamaForCausalLM", "Kuponex", "Sepedra"])
+@pytest.mark.parametrize("weight_dtype", ["float8", "bfloat16"])
+def test_a_written_folder_says_whether_its_tensors_are_in_8_bits(tmp_path, name, weight_dtype):
+    folder = write_random_model(tmp_path, dict(registry.ARCHITECTURES[name].tiny_config), 3, 0.05, weight_dtype)
+    said = json.loads((folder / "config.json").read_text()).get("quantization_config")
+    stored = any(t.dtype == torch.float8_e4m3fn for t in safetensors_io.read_folder(folder).values())
+    assert stored == (weight_dtype == "float8" and name != "Sepedra")                   # (its parts take no matrix so)
+    assert said == ({"quant_method": "fp8", "fmt": "e4m3", "activation_scheme": "dynamic", "weight_block_size": [128, 128]} if stored else None)
+    raw = registry.read_model_config(folder)
+    assert loader.load_folder(folder, describe(raw)).keys() == describe(raw).keys()
+    registry.ARCHITECTURES[name].config_from_dict(raw)
