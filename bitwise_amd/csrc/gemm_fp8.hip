@@ -798,6 +798,15 @@ int gated_by_tiles(const Fp8Args& a, int shape, hipStream_t s) {
 
 bool aligned(const void* p, int n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
+// Whether a result lies in what workgroups beside its own still read: rows of codes with their scales, a matrix (``halves`` times N rows) with its.
+bool in_operands(const Lies& out, const void* x, int ldx, const float* xs, int ldxs, const void* w, const float* ws, int rows, int N, int K, int halves) {
+  const long long kb = K / BW_FP8_BLOCK, nb = (long long)halves * ((N + BW_FP8_BLOCK - 1) / BW_FP8_BLOCK);
+  const Lies operands[] = {{x, ldx, K, rows, 1}, {xs, 4ll * ldxs, 4ll * rows, kb, 4}, {w, 0, (long long)halves * N * K, 1, 1}, {ws, 0, 4 * nb * kb, 1, 4}};
+  for (const Lies& o : operands)
+    if (meet(out, o)) return true;
+  return false;
+}
+
 // sizes that every entry point refuses
 int sizes_wrong(const void* x, int ldx, int ldxs, const void* w, int rows, int N, int K) {
   if (N < 1 || K < BW_FP8_BLOCK || K % BW_FP8_BLOCK || K > (1 << 22) || N > (1 << 24) || rows > (1 << 22) || (rows > 1 && ldx < K) || ldxs < rows) return -2;
@@ -813,7 +822,10 @@ extern "C" int bw_gemm_fp8(const void* x, int ldx, const float* xs, int ldxs, co
   if (rows <= 0) return 0;
   if (const int bad = sizes_wrong(x, ldx, ldxs, w, rows, N, K)) return bad;
   if (rows > 1 && (ldo < N || (residual != nullptr && ldr < N))) return -2;
-  if ((out_is_bf16 && residual != nullptr) || out == x) return -2;                    // (x: other workgroups still read it)
+  if (out_is_bf16 && residual != nullptr) return -2;
+  const int size = out_is_bf16 ? 2 : 4;
+  const Lies at_out = {out, (long long)ldo * size, (long long)N * size, rows, size}, at_residual = {residual, 4ll * ldr, 4ll * N, rows, 4};
+  if (in_operands(at_out, x, ldx, xs, ldxs, w, ws, rows, N, K, 1) || !in_place_or_apart(at_out, at_residual)) return -2;
   Fp8Args a = {};
   a.x = (const uint8_t*)x, a.xs = xs, a.w = (const uint8_t*)w, a.ws = ws, a.residual = residual, a.out = out;
   a.ldx = ldx, a.ldxs = ldxs, a.ldr = ldr, a.ldo = ldo, a.M = rows, a.N = N, a.K = K;
@@ -844,14 +856,19 @@ extern "C" int bw_gemm_fp8_swiglu(const void* x, int ldx, const float* xs, int l
   if (rows <= 0) return 0;
   if (const int bad = sizes_wrong(x, ldx, ldxs, w, rows, inter, K)) return bad;
   const int whole = (inter + BW_FP8_BLOCK - 1) / BW_FP8_BLOCK * BW_FP8_BLOCK;
-  if ((rows > 1 && ldq < whole) || lds < rows || codes == x || scales == xs) return -2;   // (x: other workgroups still read it)
+  if ((rows > 1 && ldq < whole) || lds < rows) return -2;
+  if (rows <= FEW_ROWS && (sums == nullptr || (rows > 1 && ldsums < inter))) return -2;
   if (!aligned(codes, 16) || ldq % 16) return -3;
+  const Lies results[] = {{codes, ldq, whole, rows, 1}, {scales, 4ll * lds, 4ll * rows, whole / BW_FP8_BLOCK, 4},
+                          {rows <= FEW_ROWS ? sums : nullptr, 4ll * ldsums, 4ll * inter, rows, 4}};
+  for (const Lies& r : results)
+    if (in_operands(r, x, ldx, xs, ldxs, w, ws, rows, inter, K, 2)) return -2;
+  if (meet(results[0], results[1]) || meet(results[0], results[2]) || meet(results[1], results[2])) return -2;
   Fp8Args a = {};
   a.x = (const uint8_t*)x, a.xs = xs, a.w = (const uint8_t*)w, a.ws = ws;
   a.ldx = ldx, a.ldxs = ldxs, a.M = rows, a.N = inter, a.K = K;
   hipStream_t s = (hipStream_t)stream;
   const Choice c = choose_gated(rows, inter, K);
-  if (rows <= FEW_ROWS && (sums == nullptr || (rows > 1 && ldsums < inter))) return -2;
   if (c.strips >= 0) {
     a.out = sums, a.ldo = ldsums;
     if (const int bad = by_strips<SWIGLU_F32>(a, c.strips, s)) return bad;

@@ -2134,7 +2134,7 @@ def quantize_fp8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, row
 
     with quotients rounded to 32 bits once, the codes to nearest even.  ``codes`` [>= rows, fp8_width(K)] gets zeros behind the rows' end;
     ``scales`` [fp8_width(K) / 128, >= rows].  A block that holds an infinity or NaN stands for NaN throughout.
-    ``codes`` is memory of its own."""
+    ``codes`` and ``scales`` share no memory with ``x``."""
     if x.dtype not in (_BF16, _F32) or x.dim() != 2:
         raise ValueError(f"quantize_fp8: x must be a bfloat16 or float32 matrix, got {x.dtype}")
     device, width = _device_of(x, "quantize_fp8: x"), x.shape[1]
@@ -2155,7 +2155,8 @@ def norm_add_norm(x: torch.Tensor, y: Optional[torch.Tensor], weight: torch.Tens
     bfloat16 or float32; ``gate`` [rows, dim] or [dim], ``scale`` a number or a vector [dim], the weights [dim]: bfloat16 or
     float32 each.  ``stream`` (float32) may be x and is x if not given.  ``out`` is float32, bfloat16 (one rounding) or e4m3
     codes [rows, fp8_width(dim)] with ``scales`` as ``quantize_fp8`` of the 32-bit rows gives them.  y None: out = norm(x) *
-    weight, and nothing else is given."""
+    weight, and nothing else is given.  Results may be x, y or a row gate themselves (of their type, with their stride); otherwise they
+    share no memory with what is read, nor with one another."""
     if x.dim() != 2:
         raise ValueError("norm_add_norm: x must be a matrix")
     device, dim = _device_of(x, "norm_add_norm: x"), x.shape[1]
@@ -2199,8 +2200,8 @@ def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales:
     ``w`` [N, fp8_width(K)] with zeros behind K and ``w_scales`` [ceil(N / 128), fp8_width(K) / 128], a scale for each 128 x 128
     block.  Each block's products are summed in 32 bits, the blocks' sums times their two scales are added up in 32 bits, k
     ascending: a row's bits do not depend on the rows beside it.  ``out`` is float32 or bfloat16 (one rounding), its rows a stride
-    apart; ``residual`` (float32, with a float32 ``out``, which it may be) is added last.  ``out`` shares no memory with
-    ``x``."""
+    apart; ``residual`` (float32, with a float32 ``out``, which it may be, with its stride) is added last.  Apart from that
+    ``out`` shares no memory with what is read."""
     device = _device_of(x, "gemm_fp8: x")
     xp, ldx, sp, lds, blocks = _codes_arg(x, x_scales, rows, None, device, "gemm_fp8")
     wp, wsp, n = _fp8_matrix_arg(w, w_scales, 1, blocks, device, "gemm_fp8")
@@ -2227,7 +2228,7 @@ def gemm_fp8_swiglu(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_
     ready for the product with its down projection.  ``w`` [2N, K] holds the gate rows, then the up rows, each half with scale
     blocks of its own: ``w_scales`` [2 ceil(N / 128), K / 128].  More than 64 rows: one launch, whose epilogue does it all; up to 64
     rows need ``sums`` (float32 [>= rows, N]), where silu(g) * u lies between two launches.  The bits are the same either way.
-    What comes out shares no memory with what goes in."""
+    What comes out, ``sums`` too, shares no memory with what goes in, nor with one another."""
     device = _device_of(x, "gemm_fp8_swiglu: x")
     xp, ldx, sp, lds, blocks = _codes_arg(x, x_scales, rows, None, device, "gemm_fp8_swiglu")
     wp, wsp, n = _fp8_matrix_arg(w, w_scales, 2, blocks, device, "gemm_fp8_swiglu")

@@ -199,8 +199,11 @@ extern "C" int bw_quantize_fp8(const void* x, int x_is_bf16, int ldx, void* code
   const long long blocks = ((long long)width + BW_FP8_BLOCK - 1) / BW_FP8_BLOCK;
   if (width < 1 || blocks > 0x7fffff || (rows > 1 && (ldx < width || ldq < blocks * BW_FP8_BLOCK)) || lds < rows || rows > 16 * 65535) return -2;
   if (!aligned16(codes) || ldq % 16) return -3;
-  if (x == codes) return -2;                                     // (rows that others still read would be written over)
   const int size = x_is_bf16 ? 2 : 4;
+  // (rows that others still read would be written over)
+  const Lies at_x = {x, (long long)ldx * size, (long long)width * size, rows, size}, at_codes = {codes, ldq, blocks * BW_FP8_BLOCK, rows, 1},
+             at_scales = {scales, 4ll * lds, 4ll * rows, blocks, 4};
+  if (meet(at_codes, at_x) || meet(at_scales, at_x) || meet(at_scales, at_codes)) return -2;
   const bool vec = aligned16(x) && width % 8 == 0 && (rows == 1 || (long long)ldx * size % 16 == 0);
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, (unsigned)((rows + 15) / 16)), dim3(256), 0, (hipStream_t)stream, x, x_is_bf16, ldx,
@@ -218,11 +221,25 @@ extern "C" int bw_norm_add_norm(const float* x, int ldx, const void* y, int y_is
   if (rows <= 0) return 0;
   if (dim < 1 || dim > (1 << 30) || rows > (1 << 21) || out_kind < 0 || out_kind > 2 || (y != nullptr && stream_out == nullptr) || (out_kind == OUT_FP8 && (scales == nullptr || lds < rows)))
     return -2;
-  if (y != nullptr && out == stream_out) return -2;              // (two results, one place)
   const int ends = out_kind == OUT_FP8 ? (dim + BW_FP8_BLOCK - 1) / BW_FP8_BLOCK * BW_FP8_BLOCK : dim;
   if (rows > 1 && (ldx < dim || ldo < ends || (y != nullptr && (ldy < dim || ldst < dim)) || (gate != nullptr && ldg != 0 && ldg < dim))) return -2;
   if (y == nullptr && (post_weight != nullptr || gate != nullptr || scale_vec != nullptr)) return -2;
   if (out_kind == OUT_FP8 && (!aligned16(out) || ldo % 16)) return -3;
+  // A row is read before it is written, by one workgroup: results may lie in the place of what is read element by element, and nowhere else in it
+  // (other workgroups still read the rows there), nor in one another.
+  const int out_size = out_kind == OUT_FP8 ? 1 : out_kind == OUT_BF16 ? 2 : 4;
+  auto rows_at = [&](const void* p, long long ld, long long n, int size) { return Lies{p, ld * size, n * size, rows, size}; };
+  auto vector_at = [&](const void* p, int bf16) { return Lies{p, 0, (long long)dim * (bf16 ? 2 : 4), 1, bf16 ? 2 : 4}; };
+  const Lies at_out = rows_at(out, ldo, ends, out_size), at_stream = rows_at(y != nullptr ? stream_out : nullptr, ldst, dim, 4),
+             at_scales = {out_kind == OUT_FP8 ? scales : nullptr, 4ll * lds, 4ll * rows, (ends + BW_FP8_BLOCK - 1) / BW_FP8_BLOCK, 4};
+  const Lies by_element[] = {rows_at(x, ldx, dim, 4), rows_at(y, ldy, dim, y_is_bf16 ? 2 : 4), rows_at(ldg != 0 ? gate : nullptr, ldg, dim, gate_is_bf16 ? 2 : 4)};
+  const Lies by_all[] = {vector_at(weight, weight_is_bf16), vector_at(post_weight, post_is_bf16), vector_at(scale_vec, scale_is_bf16),
+                         vector_at(ldg == 0 ? gate : nullptr, gate_is_bf16)};
+  if (meet(at_out, at_stream) || meet(at_scales, at_out) || meet(at_scales, at_stream)) return -2;
+  for (const Lies& in : by_element)
+    if (!in_place_or_apart(at_out, in) || !in_place_or_apart(at_stream, in) || meet(at_scales, in)) return -2;
+  for (const Lies& in : by_all)
+    if (meet(at_out, in) || meet(at_stream, in) || meet(at_scales, in)) return -2;
   NormAddNormArgs a;
   a.x = x, a.y = y, a.post_weight = post_weight, a.gate = gate, a.scale_vec = scale_vec, a.weight = weight, a.stream = stream_out, a.out = out, a.scales = scales;
   a.ldx = ldx, a.ldy = ldy, a.ldg = ldg, a.ldst = ldst, a.ldo = ldo, a.lds = lds;

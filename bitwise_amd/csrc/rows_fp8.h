@@ -121,3 +121,29 @@ __device__ __forceinline__ float sigmoid32(float g) { return g != g ? g : sigmoi
 
 // silu(g) u (a NaN goes through the first product)
 __device__ __forceinline__ float silu32_times(float g, float u) { return (g * sigmoid_of_number(g)) * u; }
+
+// ------------------------------------------------------------------------------ where a call's matrices lie (host)
+
+// ``rows`` rows of ``wide`` bytes that begin ``apart`` bytes from one another, in elements of ``size`` bytes; at null: not there.
+struct Lies {
+  const void* at;
+  long long apart, wide;
+  long long rows;
+  int size;
+};
+
+// Whether two share memory.  Rows an equal distance apart may lie beside one another, as columns of one wider matrix.
+static inline bool meet(const Lies& a, const Lies& b) {
+  if (a.at == nullptr || b.at == nullptr || a.rows < 1 || b.rows < 1) return false;
+  const long long a0 = (long long)(uintptr_t)a.at, b0 = (long long)(uintptr_t)b.at;
+  if (a0 + (a.rows - 1) * a.apart + a.wide <= b0 || b0 + (b.rows - 1) * b.apart + b.wide <= a0) return false;
+  const long long apart = a.rows > 1 ? a.apart : b.apart;
+  if ((a.rows == 1 && b.rows == 1) || (a.rows > 1 && b.rows > 1 && a.apart != b.apart) || apart <= 0) return true;
+  const long long behind = ((b0 - a0) % apart + apart) % apart;
+  return behind < a.wide || behind + b.wide > apart;
+}
+
+// Whether an output keeps out of what a kernel reads element by element: apart from it, or in its place, element for element.
+static inline bool in_place_or_apart(const Lies& out, const Lies& in) {
+  return !meet(out, in) || (out.at == in.at && out.size == in.size && out.wide == in.wide && (out.rows == 1 || out.apart == in.apart));
+}

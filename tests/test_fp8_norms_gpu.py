@@ -76,3 +76,35 @@ def test_codes_that_start_between_16_bytes_are_refused(gpu):
                 call()
     ops.gemm_fp8(good, s, w, ws, out, 4)
     assert not out.any() and not wide.view(torch.uint8).any()
+
+
+def test_results_in_the_place_of_what_is_read(gpu):
+    """Element for element they may lie there, and beside it as columns of one matrix; the bits are those of memory of its own."""
+    for dim in (256, 9000):
+        g = torch.Generator().manual_seed(dim)
+        x, y, gate = (torch.randn(5, dim, generator=g).to(gpu) for _ in range(3))
+        w = torch.ones(dim, device=gpu)
+        stream, out = torch.empty_like(x), torch.empty_like(x)
+        ops.norm_add_norm(x, y, w, out, 5, 1e-6, post_weight=w, gate=gate, scale=0.5, stream=stream)
+        for where_s, where_o in (("x", None), ("y", None), ("gate", None), (None, "x"), (None, "y"), (None, "gate"), ("y", "x"), ("x", "gate")):
+            t = {"x": x.clone(), "y": y.clone(), "gate": gate.clone(), None: torch.empty_like(x)}
+            s, o = t[where_s], t[where_o] if where_o else torch.empty_like(x)
+            ops.norm_add_norm(t["x"], t["y"], w, o, 5, 1e-6, post_weight=w, gate=t["gate"], scale=0.5, stream=s)
+            assert torch.equal(s, stream) and torch.equal(o, out), (where_s, where_o)
+        half = y.bfloat16()
+        rounded = torch.empty_like(half)
+        ops.norm_add_norm(x, half, w, rounded, 5, 1e-6, stream=stream)
+        ops.norm_add_norm(x, half, w, half, 5, 1e-6, stream=stream)
+        assert torch.equal(half, rounded)
+        wide = torch.cat([x, y, gate, x], dim=1)
+        part = [wide[:, i * dim:(i + 1) * dim] for i in range(4)]
+        ops.norm_add_norm(x, y, w, out, 5, 1e-6, gate=gate, stream=stream)
+        ops.norm_add_norm(part[0], part[1], w, part[3], 5, 1e-6, gate=part[2], stream=part[0])
+        assert torch.equal(part[0], stream) and torch.equal(part[3], out) and torch.equal(part[1], y) and torch.equal(part[2], gate)
+        alone, again = x.clone(), torch.empty_like(x)
+        ops.norm_add_norm(x, None, w, again, 5, 1e-6)
+        ops.norm_add_norm(alone, None, w, alone, 5, 1e-6)
+        assert torch.equal(alone, again)
+        with pytest.raises(RuntimeError, match="norm_add_norm"):
+            ops.norm_add_norm(x, None, w, x.view(torch.bfloat16)[:, :dim], 5, 1e-6)
+        assert torch.equal(part[1], y)
