@@ -2023,6 +2023,7 @@ def moe_combine(y: torch.Tensor, place: torch.Tensor, wts: torch.Tensor, top: in
 FP8 = torch.float8_e4m3fn
 FP8_BLOCK = 128                # elements of a row (rows and elements of a matrix) that share a scale
 FP8_SUMS_ROWS = 64             # rows up to which ``gemm_fp8_swiglu`` needs its buffer
+_INT_END = 2 ** 31             # sizes and strides go to the kernels in 32 bits
 
 
 def fp8_width(width: int) -> int:
@@ -2054,7 +2055,7 @@ def _matrix_arg(t: torch.Tensor, rows: int, width: int, device: int, what: str, 
     if (dtype is _F32 or (dtype is _BF16 and not f32_only)) and t.dim() == 2:
         n, w = t.shape
         ld, inner = t.stride()
-        if n >= rows and w == width and (inner == 1 or w == 1) and t.get_device() == device:
+        if n >= rows and w == width and (inner == 1 or w == 1) and t.get_device() == device and rows < _INT_END and w < _INT_END and (ld < _INT_END or rows <= 1):
             return t.data_ptr(), ld if rows > 1 else w, dtype is _BF16
     if dtype != _BF16 or f32_only:
         _need_rows(t, _F32, what)
@@ -2062,6 +2063,8 @@ def _matrix_arg(t: torch.Tensor, rows: int, width: int, device: int, what: str, 
         _need_rows(t, _BF16, what)
     if t.shape[0] < rows or t.shape[1] != width:
         raise ValueError(f"{what} {tuple(t.shape)} does not fit {rows} rows of {width}")
+    if rows >= _INT_END or width >= _INT_END or t.stride(0) >= _INT_END:
+        raise ValueError(f"{what}: rows, their width and the elements between them stay under 2^31")
     raise ValueError(f"{what}: all tensors live on the current device")
 
 
@@ -2084,7 +2087,8 @@ def _codes_arg(codes: torch.Tensor, scales: torch.Tensor, rows: int, width: Opti
         lb, one = scales.stride()
         at = codes.data_ptr()
         if (n >= rows and r >= rows and k == blocks * FP8_BLOCK and k > 0 and inner == 1 and (one == 1 or r == 1) and at % 16 == 0
-                and (ld % 16 == 0 or rows <= 1) and (width is None or k - FP8_BLOCK < width <= k)
+                and (rows <= 1 or (ld % 16 == 0 and ld < _INT_END)) and k < _INT_END and (lb < _INT_END or blocks <= 1) and r < _INT_END
+                and (width is None or k - FP8_BLOCK < width <= k)
                 and codes.get_device() == device and scales.get_device() == device):
             return at, ld if rows > 1 else k, scales.data_ptr(), lb if blocks > 1 else r, blocks
     _need_rows(codes, FP8, f"{what}: codes")
@@ -2097,6 +2101,8 @@ def _codes_arg(codes: torch.Tensor, scales: torch.Tensor, rows: int, width: Opti
         raise ValueError(f"{what}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} (blocks by rows) do not fit {rows} rows")
     if codes.data_ptr() % 16 or (rows > 1 and codes.stride(0) % 16):
         raise ValueError(f"{what}: rows of codes start at multiples of 16 bytes")
+    if max(rows, *codes.shape, *codes.stride(), *scales.shape, *scales.stride()) >= _INT_END:
+        raise ValueError(f"{what}: rows, their width and the elements between them stay under 2^31")
     raise ValueError(f"{what}: all tensors live on the current device")
 
 
