@@ -259,6 +259,8 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
           if (g == 0) factor[(wave * NB + b) * (WM * 16) + 16 * i + r] = both[i][b];
         }
       }
+    } else if constexpr (VIA != STRAIGHT) {
+      __builtin_amdgcn_s_waitcnt(vmcnt_only(0));                 // (its last loads still go to the workgroup's LDS: not behind its end)
     }
     if (!LAST && VIA == STRAIGHT) issue(pass + 1);
     lds_barrier();
