@@ -102,8 +102,10 @@ __device__ __forceinline__ void store_one(const Fp8Args& a, int m, int n, float 
 
 // ------------------------------------------------------------------------------ few rows
 
-// Offsets behind the descriptors of up to 64 rows (of at most 2^23 bytes), whose sums stay below 2^31.
-constexpr int FAR = 0x40000000, BEHIND = 0x30000000;
+// What lies outside of what is read is told by a lane's own offset (behind the descriptor, whatever the scalar offset adds: rows past the
+// matrices) or by a descriptor without a byte (blocks past K), never by the scalar offset, which not every range check counts.
+// FAR: behind the descriptors of up to 64 rows of at most 2^23 bytes, with room for a strip's offset below 2^31.
+constexpr int FAR = 0x40000000;
 
 // How a wave gets its block's rows: straight into registers as the matrix instructions take them, or by way of LDS (a room of its own,
 // 128 bytes a row as in the tiles below), where each load brings eight whole rows; ROOM8: with room for eight rows of x only.
@@ -135,13 +137,12 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
   const int n0 = (8 * of_eight + (int)(blockIdx.x & 7)) * (CW * NC), m0 = (int)(blockIdx.x / 8 - of_eight * a.m_tiles) * (16 * WM), KB = a.K / BW_FP8_BLOCK;
   if (n0 >= a.N) return;
   const int rows = min(16 * WM, a.M - m0);
-  __amdgpu_buffer_rsrc_t rs_w[NB], rs_ws[NB];
+  __amdgpu_buffer_rsrc_t rs_ws[NB];
+  const int size_w = min(CW * NC, a.N - n0) * a.K, size_x = (rows - 1) * a.ldx + a.K;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    rs_w[b] = rows_of(a.w + ((size_t)b * a.N + n0) * a.K, (size_t)min(CW * NC, a.N - n0) * a.K);
     rs_ws[b] = rows_of(a.ws + ((size_t)(n0 / BW_FP8_BLOCK) + (size_t)b * ((a.N + BW_FP8_BLOCK - 1) / BW_FP8_BLOCK)) * KB, (size_t)KB * 4);
   }
-  const __amdgpu_buffer_rsrc_t rs_x = rows_of(a.x + (size_t)m0 * a.ldx, (size_t)(rows - 1) * a.ldx + a.K);
   int row_m[WM];
 #pragma unroll
   for (int i = 0; i < WM; ++i) row_m[i] = m0 + min(16 * i + r, rows - 1);
@@ -169,11 +170,16 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
   // All are vector loads, in one order everywhere and in the last pass not at all, so that what is waited for is never more than
   // needed.  Factors last were slower, 64 x 6144 x 4096 18.3 for 16.6.)
   auto issue = [&](int pass) {
-    const int blk = pass * NW + wave, at_k = blk < KB ? blk * BW_FP8_BLOCK : BEHIND;
+    const int blk = pass * NW + wave, here = min(blk, KB - 1), at_k = here * BW_FP8_BLOCK;
+    const bool live = blk < KB;
+    const __amdgpu_buffer_rsrc_t rs_x = rows_of(a.x + (size_t)m0 * a.ldx, live ? size_x : 0);
+    __amdgpu_buffer_rsrc_t rs_w[NB];
 #pragma unroll
-    for (int i = 0; i < WM; ++i) sx[i] = a.xs[(size_t)min(blk, KB - 1) * a.ldxs + row_m[i]];
+    for (int b = 0; b < NB; ++b) rs_w[b] = rows_of(a.w + ((size_t)b * a.N + n0) * a.K, live ? size_w : 0);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) sw[b] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs_ws[b], 0, blk * 4, 0));
+    for (int i = 0; i < WM; ++i) sx[i] = a.xs[(size_t)here * a.ldxs + row_m[i]];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) sw[b] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs_ws[b], 0, here * 4, 0));
     if constexpr (VIA == STRAIGHT) {
 #pragma unroll
       for (int c = 0; c < NC; ++c)
@@ -191,11 +197,11 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_few_kernel(Fp8Args a) {
     } else {
       // (rows past the matrices lie outside the descriptors: zeros)
 #pragma unroll
-      for (int t = 0; t < BX; ++t) load_to_lds(rs_x, mine + t * 1024, via_x[t & 1], at_k + 8 * t * a.ldx);
+      for (int t = 0; t < BX; ++t) load_to_lds(rs_x, mine + t * 1024, via_x[t & 1] + 8 * t * a.ldx, at_k);
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int t = 0; t < BW / NB; ++t) load_to_lds(rs_w[b], mine + (BX + b * (BW / NB) + t) * 1024, via_w[CW == 16 ? t & 1 : 0], at_k + 8 * t * a.K);
+        for (int t = 0; t < BW / NB; ++t) load_to_lds(rs_w[b], mine + (BX + b * (BW / NB) + t) * 1024, via_w[CW == 16 ? t & 1 : 0] + 8 * t * a.K, at_k);
     }
     __builtin_amdgcn_sched_barrier(0);
   };
