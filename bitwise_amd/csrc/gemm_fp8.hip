@@ -93,7 +93,9 @@ __device__ __forceinline__ void store_one(const Fp8Args& a, int m, int n, float 
   if constexpr (EPI == STORE_BF16) {
     ((bf16_t*)a.out)[(size_t)m * a.ldo + n] = f32_to_bf16(y);
   } else if constexpr (EPI == SWIGLU_F32) {
-    ((float*)a.out)[(size_t)m * a.ldo + n] = silu32_times(y, u);
+    // (a NaN goes through the first product)
+    with_sigmoids<1>([&](int) { return y; }, [&](int, float s) { y = (y * s) * u; });
+    ((float*)a.out)[(size_t)m * a.ldo + n] = y;
   } else {
     if (a.residual != nullptr) y = a.residual[(size_t)m * a.ldr + n] + y;
     ((float*)a.out)[(size_t)m * a.ldo + n] = y;
@@ -561,13 +563,11 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       uint32_t mx = 0u;
+      with_sigmoids<4 * NH>([&](int k) { return acc[i][k / 4][k % 4]; }, [&](int k, float s) {
+        acc[i][k / 4][k % 4] = (acc[i][k / 4][k % 4] * s) * acc[i][NH + k / 4][k % 4];
+      });
 #pragma unroll
-      for (int j = 0; j < NH; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          acc[i][j][q] = silu32_times(acc[i][j][q], acc[i][NH + j][q]);
-          mx = max_bits(mx, __float_as_uint(acc[i][j][q]) & 0x7fffffffu);
-        }
+      for (int k = 0; k < 4 * NH; ++k) mx = max_bits(mx, __float_as_uint(acc[i][k / 4][k % 4]) & 0x7fffffffu);
       float lo, hi;
       lane_halves<32>(__uint_as_float(mx), lo, hi);
       mx = max_bits(__float_as_uint(lo), __float_as_uint(hi));
