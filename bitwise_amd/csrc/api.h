@@ -322,7 +322,7 @@ int bw_norm_add_norm(const float* x, int ldx, const void* y, int y_is_bf16, int 
 int bw_gemm_fp8(const void* x, int ldx, const float* xs, int ldxs, const void* w, const float* ws, const float* residual, int ldr, void* out,
                 int ldo, int out_is_bf16, int rows, int N, int K, void* stream);
 // Which kernels a product's sizes lead to: choice[0] strips (100: those for up to 16 rows) or -1 and choice[1] tiles, choice[2] the rows
-// behind the tiles that go by strips.
+// behind the tiles that a launch of their own takes, by what so many rows alone lead to.
 int bw_gemm_fp8_choice(int rows, int N, int K, int gated, int* choice);
 // codes, scales = quantized silu(g) u with [g | u] = x w^T: w [2 inter, K] (gate rows, then up rows), each half with scale blocks of
 // its own.  Up to 64 rows: ``sums`` [rows, inter] holds silu(g) u between two launches; more rows do not touch it.

@@ -742,12 +742,14 @@ constexpr ShapeCost GATED_STRIPS[] = {{32, 16, 2, 0.0, 0.285, 0.0, 0.47}, {32, 3
 constexpr ShapeCost STORE_TILES[] = {{192, 256, 1, 6.5, 2.04, 0, 0}, {128, 128, 2, 5.8, 1.02, 6.5, 1.78}, {64, 128, 2, 2.9, 0.64, 3.1, 1.12}, {64, 64, 2, 2.5, 0.49, 3.2, 0.74}};
 constexpr ShapeCost GATED_TILES[] = {{192, 128, 1, 11.0, 2.04, 0, 0}, {128, 128, 1, 5.5, 1.70, 0, 0}, {64, 128, 2, 3.5, 1.20, 9.5, 1.60}, {32, 128, 2, 2.5, 0.95, 4.5, 1.30}};
 
-constexpr int STRIPS_MOST_ROWS = 1024;          // (the grid's second size stays small; far more rows are always cheaper by tiles)
+// The strips' prices hold for rounds of few rows; past this, products of few columns are as often faster by tiles (30 of them, 1,037 to 9,662 rows of
+// 27 to 407 columns: by strips 1.08 of the time, 0.5 to 2.2 one by one).
+constexpr int STRIPS_MOST_ROWS = 1024;
 
 constexpr int FEW_ROWS = 64;                    // rows up to which a gated product has a buffer for its sums
 
 // What runs: ``strips`` (of the tables above; SIXTEEN: up to 16 rows, the strips made for those), or -1 and ``tiles``, the last ``tail``
-// rows behind the tiles by strips of their own.
+// rows behind the tiles by a launch of their own, which takes what a product of so many rows takes (``choose_stored`` again).
 struct Choice {
   int strips, tiles, tail;
 };
@@ -758,8 +760,11 @@ Choice choose_stored(int rows, int N, int K) {
   int shape = cheapest(STORE_TILES, rows, N, K, &us), tail = 0;
   const int strips = cheapest(STORE_STRIPS, rows, N, K, &strips_us);
   if (rows > STRIPS_MOST_ROWS) strips_us = us + 1.0;
-  // A few rows past whole tiles can cost a round of their own: then they go by strips, behind the tiles (777 x 5003 x 2000, of which 768
-  // rows are one round, 35.9 -> 32.7 us; 2100 x 2048 x 2048 31.5 -> 27.5).
+  // A few rows past whole tiles can cost a round of their own: then they go behind the tiles (777 x 5003 x 2000, of which 768 rows are one
+  // round, 35.9 -> 32.7 us; 2100 x 2048 x 2048 31.5 -> 27.5).  Their price is that of strips, also where they then take small tiles (one such
+  // launch in eight): priced as those, which a table of whole products puts too low behind others, 40 products that change took 1.07 of the time;
+  // by strips after all, 40 such products took 1.03.  Up to 16 rows run strips that have no table: over 45 sizes 0.74 to 1.33 of the price, 1.08 in
+  // the middle.
   double best = us < strips_us ? us : strips_us;
   for (int i = 0; i < 4; ++i) {
     const int rest = rows % STORE_TILES[i].rows;

@@ -2222,7 +2222,7 @@ def gemm_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales:
 
 def gemm_fp8_choice(rows: int, n: int, k: int, gated: bool = False) -> Tuple[int, int, int]:
     """Which kernels a product of these sizes (``k`` in whole blocks) runs, see gemm_fp8.hip: (strips, or -1; tiles; rows behind the
-    tiles that go by strips)."""
+    tiles that a launch of their own takes, by what so many rows alone lead to)."""
     out = (c_int * 3)()
     _check(_fn("bw_gemm_fp8_choice")(int(rows), int(n), int(k), int(gated), ctypes.cast(out, c_void_p)), "gemm_fp8_choice")
     return tuple(out)
