@@ -660,15 +660,16 @@ int launch_few(Fp8Args a, hipStream_t s) {
 // one (4 of 4096, K = 14336: 12.7, with eight 14.2).  Up to 2048 columns strips of eight, so that every unit has one: of 2048
 // columns, K = 8192, 6.4 us for 7.2; by eight waves where K has no work for more (K = 1024 2.7 for 2.9).  Up to eight rows leave eight waves room for
 // a fourth workgroup a unit (2 x 16384 x 8192 30.1 -> 27.6 us); with sixteen, one a unit is better (4 x 4096 x 14336 12.7 for 14.5).
-// Two strips a workgroup share x where there is more of it and K is short (16 x 28672 x 2048 15.1 -> 14.2, 16 x 6144 x 4096 9.2 -> 8.5; 16 x 8192 x
-// 8192 16.4 -> 17.2), or where one workgroup a unit then takes all (8 x 6144 x 4096 8.8 -> 8.0 on inputs from memory, gated 3 x 5504 x 2048 9.8 -> 9.0;
-// 1 x 28672 x 4096 24.2 -> 25.0).
+// Two strips a workgroup share x where there is more of it (16 x 28672 x 2048 14.8 -> 14.0, 16 x 6144 x 5120 11.6 -> 10.5, 16 x 28672 x 14336 89.9 ->
+// 80.8), or where one workgroup a unit then takes all (8 x 6144 x 5120 9.8 -> 9.4, gated 3 x 5504 x 2048 9.8 -> 9.0; 1 x 28672 x 4096 24.2 -> 25.0).  Not
+// where the matrix's rows lie a multiple of 8,192 bytes apart, so that twice as many of them meet in the same channels (12 x 8192 x 8192 15.9 ->
+// 17.3, 8 x 6144 x 8192 13.2 -> 14.2, 16 x 20000 x 16384 67 -> 73; K = 8064 and 8320 gain 1.03 to 1.13, 12288 0.94 to 1.06, 24576 0.96 to 1.09).
 template <int EPI, int VIA>
 int sixteen_rows(const Fp8Args& a, hipStream_t s) {
   if constexpr (EPI != SWIGLU_F32) {
     if (a.N <= 2048) return a.K <= 8 * BW_FP8_BLOCK ? launch_few<1, 1, EPI, 8, 8, VIA>(a, s) : launch_few<1, 1, EPI, 16, 8, ROOM16>(a, s);
     if (a.N <= 4096) return launch_few<1, 1, EPI, 16, 16, ROOM16>(a, s);
-    if (a.K <= 4096 && (VIA == ROOM16 || a.N <= 8192)) return launch_few<1, 2, EPI, 8, 16, VIA>(a, s);
+    if (a.K % 8192 != 0 && (VIA == ROOM16 || a.N <= 8192)) return launch_few<1, 2, EPI, 8, 16, VIA>(a, s);
   } else {
     if (a.N > 4096 && a.N <= 8192) return launch_few<1, 2, EPI, 8, 16, VIA>(a, s);
   }
