@@ -114,3 +114,33 @@ def test_models_whose_feed_forwards_alone_are_in_8_bits(gpu, tmp_path, name):
         want = wide.logits(toks)
         # (a code is off by 2^-4 of its value at most, their errors do not all point one way, and the stream carries most of a logit)
         assert np.linalg.norm(whole[rid] - want) <= 2.0 ** -3 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("name", ["LONG", "B"])
+def test_an_engine_whose_captured_steps_hold_products_back(gpu, tmp_path, name):
+    """8-bit operators among products that captured steps send as phases of a few launches (the head's, and the matrices that are not in 8
+    bits): each comes behind what was held back, and the tokens and fingerprints are the ones of eager steps."""
+    import json
+
+    import bitwise_amd as bw
+    import tiny
+    from bitwise_amd.model import describe
+    from bitwise_amd.weights import loader, safetensors_io
+
+    cfg, seed, sigma, page = tiny.CONFIGS[name]
+    for stored in (("proj",), ("down_proj",), ("q_proj", "k_proj", "v_proj"), ("gate_proj", "up_proj")):
+        tensors = []
+        for n, t in loader.random_tensors(describe(cfg), seed, sigma, torch.float32):
+            tensors += list(loader.stored_as(n, describe(cfg)[n], t, block_scaled.DTYPE if any(s in n for s in stored) else torch.bfloat16))
+        folder = tmp_path / stored[0]
+        folder.mkdir()
+        (folder / "config.json").write_text(json.dumps(cfg))
+        safetensors_io.write_file(folder / "model.safetensors", tensors)
+        model = bw.Model.load(folder)
+        prompts = list(requests_for(cfg["vocab_size"], 9, [33, 8, 21, 5]).values())
+        sp = bw.SamplingParams(max_new_tokens=10, ignore_eos=True)
+        runs = [bw.generate(model, prompts, sp, bw.EngineConfig(num_blocks=64, block_size=page, max_batched_tokens=48, **kw))
+                for kw in (dict(decode_phases=True), dict(decode_phases=False), dict(use_graphs=False))]
+        for other in runs[1:]:
+            assert [r.tokens for r in runs[0]] == [r.tokens for r in other]
+            assert [r.logits_fingerprint for r in runs[0]] == [r.logits_fingerprint for r in other]
