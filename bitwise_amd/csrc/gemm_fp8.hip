@@ -322,8 +322,8 @@ __device__ __forceinline__ float taken(float v) {
 // bytes to 16 l; slot c' of row r (within its block of 16 rows) holds the row's chunk c' ^ (r >> 1), so that the 16 lanes that
 // read one chunk of 16 rows hit 16 different groups of banks (conflicts: 1 % of LDS's busy cycles).
 //
-// What bounds it, of 2048 rows by gated 14336 columns, K = 4096, 404 us (1.19 PFLOP/s; a plain bfloat16 product of the library reaches
-// 1.38): the matrix cores are busy 52 % of the cycles, and for 16 matrix instructions of a wave there are 55 others, of which 27 convert
+// What bounds it, of 2048 rows by gated 14336 columns, K = 4096, 407 us (1.18 PFLOP/s; in an unbroken row 450, 1.07; a plain bfloat16
+// product of the library reaches 1.38): the matrix cores are busy 51 % of the cycles, and for 16 matrix instructions of a wave there are 54 others, of which 27 convert
 // and 18 join chains.  Left out one at a time the conversions are worth 11 %, three quarters of the chains' multiply-adds 8 %, the reads
 // from LDS 13 %, the loads 13 %, all together 30 %: no one of them is the bound, and the clock falls with the matrix cores' power
 // (zeros for operands run 8 % faster).  So the tile is as large as a wave's registers allow: a step of 192 x 256 takes 2.04 us, of 128 x 128 for the same work 2.7.

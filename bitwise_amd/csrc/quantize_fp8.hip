@@ -138,7 +138,7 @@ __device__ __forceinline__ float row_inverse(float acc, float* part, int dim, fl
 // A workgroup a row.  WHOLE: as many threads as the row has eights of elements: all loads are asked for first, everything is read
 // once.  Otherwise (rows of more than 8,192) thread t has the eights t, t + 1024, ... in passes, and reads the stream back that it
 // wrote.  Memory bounds it, and for a few rows the two sums over a row, each behind a barrier: 2048 rows of 4096 with a gate and codes behind
-// them 25.8 us (109 MB: 4.2 TB/s; 256 threads with up to four eights each took 30.0), eight rows 4.2 us.
+// them 25.9 us (109 MB: 4.2 TB/s; 256 threads with up to four eights each took 30.0), eight rows 4.1 us.
 template <bool WHOLE, bool VEC>
 __global__ __launch_bounds__(1024) void norm_add_norm_kernel(NormAddNormArgs a) {
   __shared__ float part[2][16];
