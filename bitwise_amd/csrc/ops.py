@@ -27,7 +27,7 @@ HEAD_DIMS = (16, 32, 48, 64, 80, 96, 112, 128, 160, 192, 224, 256)
 PAGE_SIZES = (8, 16, 32, 64)       # tokens in a page that the attention kernels and the cache writes take
 
 _ERRORS = {
-    -2: "sizes or strides out of the kernel's range",
+    -2: "sizes or strides out of the kernel's range, or a result in memory that the call still reads",
     -3: "misaligned pointer or stride",
     -4: f"head size not compiled in (supported: {HEAD_DIMS})",
     -5: "page size not supported (a power of two from 4 to 64 is needed)",
@@ -2140,7 +2140,7 @@ def quantize_fp8(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, row
 
     with quotients rounded to 32 bits once, the codes to nearest even.  ``codes`` [>= rows, fp8_width(K)] gets zeros behind the rows' end;
     ``scales`` [fp8_width(K) / 128, >= rows].  A block that holds an infinity or NaN stands for NaN throughout.
-    ``codes`` and ``scales`` share no memory with ``x``."""
+    ``codes`` and ``scales`` share no memory with ``x``.  Up to 1,048,560 rows."""
     if x.dtype not in (_BF16, _F32) or x.dim() != 2:
         raise ValueError(f"quantize_fp8: x must be a bfloat16 or float32 matrix, got {x.dtype}")
     device, width = _device_of(x, "quantize_fp8: x"), x.shape[1]
@@ -2162,7 +2162,7 @@ def norm_add_norm(x: torch.Tensor, y: Optional[torch.Tensor], weight: torch.Tens
     float32 each.  ``stream`` (float32) may be x and is x if not given.  ``out`` is float32, bfloat16 (one rounding) or e4m3
     codes [rows, fp8_width(dim)] with ``scales`` as ``quantize_fp8`` of the 32-bit rows gives them.  y None: out = norm(x) *
     weight, and nothing else is given.  Results may be x, y or a row gate themselves (of their type, with their stride); otherwise they
-    share no memory with what is read, nor with one another."""
+    share no memory with what is read, nor with one another.  Up to 2,097,152 rows."""
     if x.dim() != 2:
         raise ValueError("norm_add_norm: x must be a matrix")
     device, dim = _device_of(x, "norm_add_norm: x"), x.shape[1]
